@@ -94,6 +94,18 @@ def _need(cond: bool, msg: str) -> None:
         raise KernelError(msg)
 
 
+def _on_current_device(what: str, *tensors) -> None:
+    """A kernel runs on the current device's stream: a tensor elsewhere is refused before its address is used there."""
+    here = None
+    for t in tensors:
+        if t is None:
+            continue
+        if here is None:
+            here = -2 if not t.is_cuda else _RAW_DEVICE() if _RAW_DEVICE is not None else torch.cuda.current_device()
+        if t.get_device() != here:
+            raise KernelError(f"{what}: a tensor on {t.device}, which is not the current CUDA device")
+
+
 _I, _F, _P, _LL = ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_longlong       # of the structures below
 
 
@@ -170,6 +182,7 @@ class CudaKernels:
                    "ifx_latent_decode", "ifx_latent_decode_supports", "ifx_latent_decode_stretch",
                    "ifx_latent_prompt", "ifx_latent_prompt_supports", "ifx_delta_chunks_supports", "ifx_delta_chunks_scan",
                    "ifx_attention_prefill_tcgen05_parts", "ifx_gemm_f32_split", "ifx_swiglu_few", "ifx_gemm_f32_split_launches",
+                   "ifx_selective_scan", "ifx_selective_inputs", "ifx_moe_route_groups",
                    "ifx_set_shared_carveout", "ifx_set_pdl"),
                   ("ifx_delta_rule_scratch_floats", "ifx_chunk_scan_scratch_floats", "ifx_delta_chunks_scratch_floats",
                    "ifx_attention_prefill_tcgen05_parts_bytes", "ifx_gemm_f32_split_scratch", "ifx_moe_sorted_scratch",
@@ -1763,6 +1776,33 @@ class CudaKernels:
         self.launches += 1
         return ids, weights
 
+    def moe_route_groups(self, z, correction, top, groups, kept, best=2, score="sigmoid", normalized=True, floor=0.0, scale=1.0):
+        """(ids int32 [T, top], weights float32 [T, top]) from router logits z [T, n] (float32, or a PartialSum): the experts lie in `groups`
+        equal groups; scores = sigmoid(z) or (`score` "softmax") softmax(z), and v = score + correction; a group's strength is the sum of its
+        `best` largest v; of the `kept` strongest groups the `top` experts with the largest v are chosen, falling; their weights are
+        the scores, with `normalized` divided by (their sum + floor), times `scale`.  Ties go to the lower index; what is
+        larger is decided in 64 bits on the float32 logits.  A v that is not a number counts as -inf; a row always gets `top` different experts of its
+        kept groups, with weights of zero where no score is above zero.  Up to 1,024 experts, 32 groups and 32 choices."""
+        if score not in ("sigmoid", "softmax"):
+            raise KernelError(f"moe_route_groups: unknown score {score!r}")
+        T, n = z.shape
+        src, splits = (z.parts, z.splits) if isinstance(z, PartialSum) else (z, 1)
+        _need(src.dtype == torch.float32 and src.is_contiguous() and (correction is None or (
+            correction.dtype == torch.float32 and correction.is_contiguous() and correction.numel() == n)),
+            "moe_route_groups: contiguous float32 logits and corrections")
+        top, groups, kept, best = int(top), int(groups), int(kept), int(best)
+        if not (0 < groups <= 32 and n % groups == 0 and n <= 1024 and 1 <= kept <= groups and 1 <= best <= n // groups
+                and 1 <= top <= min(32, kept * (n // groups))):
+            raise KernelError(f"moe_route_groups: {n} experts in {groups} groups, {kept} kept by their best {best}, {top} chosen")
+        _on_current_device("moe_route_groups", src, correction)
+        ids = torch.empty(T, top, dtype=torch.int32, device=src.device)
+        weights = torch.empty(T, top, dtype=torch.float32, device=src.device)
+        if T:
+            _check(self.lib.ifx_moe_route_groups(src, splits, correction, ids, weights, T, n, groups, kept, best, top, int(score == "softmax"),
+                                                 int(bool(normalized)), float(floor), float(scale), _stream()), "moe_route_groups")
+            self.launches += 1
+        return ids, weights
+
     def moe_experts(self, h, w_up, w_down, ids, weights, experts, out_dtype, glu=None):
         """sum over a token's choices of weight * W_down[e] relu(W_up[e] h)^2, or weight * h for e >= experts.
         w_up [experts, ff, width], w_down [experts, width, ff] in h's dtype.  `glu` = (limit, slope): w_up is
@@ -2137,6 +2177,83 @@ class CudaKernels:
                                        ctx.cu_seqlens, out, ctx.num_requests, T, int(ctx.max_span), int(width),
                                        _DT[out_dtype], _stream()), "gated_scan")
         self.launches += 1
+        return out
+
+    # ------------------------------------------- a state space with a decay for every channel and state number
+    SELECTIVE_MOST_STATES = 128
+
+    def selective_inputs(self, rows, rank, states, out_dtype, norms=None, eps=0.0):
+        """rows [T, >= rank + 2 states] (float32 or bfloat16, rows maybe further apart, or a PartialSum) hold a step's low-rank part, B and C side
+        by side: returns (the low-rank part [T, rank] in `out_dtype`, B | C float32 [T, 2 states]).  `norms` = (w_low [rank],
+        w_b [states], w_c [states]), float32 or None each: that part over its own root mean square (with `eps`), times its weight."""
+        rank, states = int(rank), int(states)
+        T, width = rows.shape
+        src, splits = (rows.parts, rows.splits) if isinstance(rows, PartialSum) else (rows, 1)
+        w_low, w_b, w_c = (None, None, None) if norms is None else norms
+        if not (0 < rank <= 8192 and 0 < states <= self.SELECTIVE_MOST_STATES and width >= rank + 2 * states):
+            raise KernelError(f"selective_inputs: a rank of {rank} and {states} states in rows of {width}")
+        _need(src.dtype in _DT and out_dtype in _DT and src.stride(-1) == 1 and (splits == 1 or src.is_contiguous())
+              and src.dtype in (torch.float32, torch.bfloat16), "selective_inputs: float32 or bfloat16 rows with unit column stride")
+        for w, n in ((w_low, rank), (w_b, states), (w_c, states)):
+            _need(w is None or (w.dtype == torch.float32 and w.is_contiguous() and w.numel() == n),
+                  "selective_inputs: norm weights are float32 of their part's size")
+        _on_current_device("selective_inputs", src, w_low, w_b, w_c)
+        low = torch.empty(T, rank, dtype=out_dtype, device=src.device)
+        bc = torch.empty(T, 2 * states, dtype=torch.float32, device=src.device)
+        if T:
+            ld = max(int(src.stride(-2)), width)                 # (a single row's stride may be anything)
+            _check(self.lib.ifx_selective_inputs(src, ld, _DT[src.dtype], splits, w_low, w_b, w_c, float(eps), low, _DT[out_dtype], bc, T, rank,
+                                                 states, _stream()), "selective_inputs")
+            self.launches += 1
+        return low, bc
+
+    @staticmethod
+    def _selective_rows(t, T, width, what):
+        """The distance between the rows of a float32 or bfloat16 operand of selective_scan."""
+        if t.dtype not in _DT or t.dim() != 2 or t.shape[0] != T or t.shape[1] != width or (t.stride(1) != 1 and width > 1):
+            raise KernelError(f"selective_scan: {what} must be float32 or bfloat16 [{T}, {width}] with unit column stride")
+        stride = t.stride(0)
+        if T > 1 and stride < width:
+            raise KernelError(f"selective_scan: the rows of {what} overlap")
+        return max(stride, width)
+
+    def selective_scan(self, x, dt, bc, log_rate, state, ctx, z=None, bias=None, skip=None, out_dtype=None):
+        """Per request and channel c a vector h of `states` float32 numbers, kept in `state` [slots, >= channels states] as [channel, state
+        number] (a slot's rows may be further apart) and moved on:
+            step = softplus(dt + bias);  h[n] <- exp(-step e^log_rate[c, n]) h[n] + step x B[n];  y = (sum_n C[n] h[n] + skip[c] x) silu(z)
+        x [T, channels], z (or None: no gate) of its dtype, dt: float32 or bfloat16, rows may be slices of wider rows; bc: float32 [T, 2 states],
+        B | C; log_rate: float32 [channels, states]; bias, skip: float32 [channels] or None.  Up to 128 states.  Returns y in
+        `out_dtype` (default x's).  The requests of a step are in slots of their own; a request without tokens keeps its state."""
+        _need(x.dim() == 2 and log_rate.dim() == 2, "selective_scan: rows [T, channels] and rates [channels, states]")
+        T, C = x.shape
+        N = log_rate.shape[1]
+        out_dtype = x.dtype if out_dtype is None else out_dtype
+        ld_x, ld_dt = self._selective_rows(x, T, C, "x"), self._selective_rows(dt, T, C, "dt")
+        ld_z = 0
+        if z is not None:
+            _need(z.dtype == x.dtype, "selective_scan: the gate has x's dtype")
+            ld_z = self._selective_rows(z, T, C, "z")
+        if not 0 < N <= self.SELECTIVE_MOST_STATES or C < 1:
+            raise KernelError(f"selective_scan: {C} channels of {N} states")
+        _need(bc.dtype == torch.float32, "selective_scan: float32 B and C")
+        ld_bc = self._selective_rows(bc, T, 2 * N, "B | C")
+        _need(out_dtype in _DT and log_rate.dtype == torch.float32 and log_rate.is_contiguous() and log_rate.shape[0] == C,
+              "selective_scan: float32 rates [channels, states], and y in float32 or bfloat16")
+        for vec in (bias, skip):
+            _need(vec is None or (vec.dtype == torch.float32 and vec.is_contiguous() and vec.numel() == C),
+                  "selective_scan: bias and skip are float32 [channels]")
+        _need(state is not None and state.dtype == torch.float32 and state.dim() == 2 and state.stride(1) == 1 and state.shape[1] >= C * N
+              and (state.shape[0] == 1 or state.stride(0) >= C * N), "selective_scan: the state does not fit the channels")
+        R = int(ctx.num_requests)
+        _need(ctx.cu_seqlens.dtype == torch.int32 and ctx.req_slot.dtype == torch.int32 and ctx.cu_seqlens.numel() > R
+              and ctx.req_slot.numel() >= R and R <= 65535, "selective_scan: int32 spans and slots of every request (up to 65,535)")
+        _on_current_device("selective_scan", x, dt, bc, log_rate, state, z, bias, skip, ctx.cu_seqlens, ctx.req_slot)
+        out = torch.empty(T, C, dtype=out_dtype, device=x.device)
+        if T and R:
+            _check(self.lib.ifx_selective_scan(x, ld_x, _DT[x.dtype], dt, ld_dt, _DT[dt.dtype], bc, ld_bc, z, ld_z, log_rate, bias, skip, state,
+                                               max(state.stride(0), C * N), ctx.req_slot, ctx.cu_seqlens, out, _DT[out_dtype], R, T,
+                                               int(ctx.max_span), C, N, _stream()), "selective_scan")
+            self.launches += 1
         return out
 
     # ---------------------------------------------------------------- sampling

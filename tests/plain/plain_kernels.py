@@ -534,6 +534,36 @@ class PlainKernels:
             state[slots[r], :width] = S.to(state.dtype)
         return (out * g * torch.sigmoid(g)).to(out_dtype)
 
+    # ------------------------------------------- a state space with a decay for every channel and state number
+    def selective_inputs(self, rows, rank, states, out_dtype, norms=None, eps=0.0):
+        """rows [T, >= rank + 2 states] cut into (its first `rank` columns in `out_dtype`, the 2 states behind them in float32), the three parts
+        RMS-normed where `norms` has a weight for them."""
+        parts = list(rows[:, :rank + 2 * states].to(self.acc).split([rank, states, states], dim=1))
+        for i, w in enumerate(norms or ()):
+            if w is not None:
+                parts[i] = parts[i] * torch.rsqrt(parts[i].square().mean(-1, keepdim=True) + eps) * w.to(self.acc)
+        return parts[0].to(out_dtype), torch.cat(parts[1:], 1).to(torch.float32)
+
+    def selective_scan(self, x, dt, bc, log_rate, state, ctx, z=None, bias=None, skip=None, out_dtype=None):
+        """h[c, n] <- exp(-step e^log_rate[c, n]) h[c, n] + step x[c] B[n] with step = softplus(dt + bias); returns
+        (sum_n C[n] h[c, n] + skip[c] x[c]) silu(z[c]); h per request in `state` [slots, >= channels states], moved on."""
+        A, (C, N) = self.acc, log_rate.shape
+        v = dt.to(A) if bias is None else dt.to(A) + bias.to(A)
+        step = torch.clamp(v, min=0) + torch.log1p(torch.exp(-v.abs()))
+        rate, xa, out = torch.exp(log_rate.to(A)), x.to(A), torch.zeros(x.shape, dtype=A, device=x.device)
+        cu, slots = ctx.cu_seqlens.tolist(), ctx.req_slot.tolist()
+        for r in range(ctx.num_requests):
+            h = state[slots[r], :C * N].to(A).view(C, N)
+            for t in range(cu[r], cu[r + 1]):
+                h = torch.exp(-step[t][:, None] * rate) * h + (step[t] * xa[t])[:, None] * bc[t, :N].to(A)
+                out[t] = h @ bc[t, N:].to(A)
+            state[slots[r], :C * N] = h.reshape(-1).to(state.dtype)
+        if skip is not None:
+            out = out + skip.to(A) * xa
+        if z is not None:
+            out = out * z.to(A) * torch.sigmoid(z.to(A))
+        return out.to(out_dtype or x.dtype)
+
     def linear_geglu(self, a, w_gate_up, bias):
         """gelu_tanh(a Wg^T + bg) * (a Wu^T + bu) with gate and up stacked."""
         both = self.linear(a, w_gate_up, bias=bias, out_dtype=self.acc)
@@ -557,6 +587,27 @@ class PlainKernels:
         choice = s if correction is None else s + correction.to(self.acc)
         ids = torch.topk(choice, top, dim=-1).indices
         return ids.to(torch.int32), torch.gather(s, 1, ids).to(torch.float32)
+
+    def moe_route_groups(self, z, correction, top, groups, kept, best=2, score="sigmoid", normalized=True, floor=0.0, scale=1.0):
+        """The `top` experts with the largest score + correction of the `kept` groups whose `best` largest sum to the most; ties to the lower
+        index; weights the scores (over their sum + floor), times scale.  In 64 bits always: a choice is not a matter of rounding."""
+        T, n = z.shape
+        zd = z.to(torch.float64)
+        s = torch.sigmoid(zd) if score == "sigmoid" else torch.where((zd == -math.inf).all(1, keepdim=True), 0.0, torch.softmax(zd, dim=-1))
+        v = s if correction is None else s + correction.to(torch.float64)
+        v = torch.where(v.isnan(), -math.inf, v).view(T, groups, n // groups)
+        strength = v.sort(dim=2, descending=True).values[:, :, :best].sum(2)
+        strength = torch.where(strength.isnan(), -math.inf, strength)
+        keep = torch.zeros(T, groups, dtype=torch.int64, device=z.device)
+        keep.scatter_(1, strength.sort(dim=1, descending=True, stable=True).indices[:, :kept], 1)
+        order = v.reshape(T, n).sort(dim=1, descending=True, stable=True).indices
+        kept_first = keep.repeat_interleave(n // groups, 1).gather(1, order).sort(dim=1, descending=True, stable=True).indices
+        ids = order.gather(1, kept_first)[:, :top]
+        w = s.gather(1, ids)
+        if normalized:
+            total = w.sum(1, keepdim=True) + floor
+            w = torch.where(total == 0, 0.0, w / total)
+        return ids.to(torch.int32), (w * scale).to(torch.float32)
 
     def moe_experts(self, h, w_up, w_down, ids, weights, experts, out_dtype, glu=None):
         """`glu` = (limit, slope[, offset = 1]): w_up holds an expert's gate rows above its up rows, and the activation is

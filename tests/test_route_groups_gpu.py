@@ -1,0 +1,105 @@
+"""Routing by groups: the choice is that of the formula in 64 bits, whatever float32 makes of an exponential."""
+import math
+
+import pytest
+import torch
+
+from plain.plain_kernels import PlainKernels
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def _same(k, z, correction, **kw):
+    on = None if correction is None else correction.to(DEV)
+    ids, w = k.moe_route_groups(z.to(DEV), on, **kw)
+    want_ids, want_w = PlainKernels().moe_route_groups(z, correction, **kw)
+    assert ids.dtype == torch.int32 and w.dtype == torch.float32
+    assert torch.equal(ids.cpu(), want_ids)
+    # 64-bit numbers rounded once, by both sides
+    assert torch.equal(w.isnan().cpu(), want_w.isnan())
+    assert bool(((w.cpu() - want_w).abs() <= want_w.abs() * 2.0 ** -23).logical_or(want_w.isnan()).all())
+    return ids, w
+
+
+@pytest.mark.parametrize("T,n,groups,kept,best,top", [
+    (24, 256, 8, 4, 2, 8), (1, 64, 8, 3, 2, 6), (333, 160, 8, 3, 1, 6), (5, 60, 4, 2, 3, 4), (70, 1024, 32, 5, 2, 32), (4, 7, 1, 1, 1, 7),
+    (9, 32, 32, 4, 1, 4), (3, 1, 1, 1, 1, 1), (17, 96, 2, 1, 48, 32), (2000, 30, 1, 1, 4, 5), (13, 72, 8, 8, 9, 8), (100, 384, 1, 1, 1, 8), (6, 1023, 3, 2, 2, 9)])
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("normalized,with_correction,scale", [(True, True, 2.5), (False, False, 1.0), (True, False, 16.0)])
+def test_choice(cuda_kernels, T, n, groups, kept, best, top, score, normalized, with_correction, scale):
+    g = torch.Generator().manual_seed(T + n)
+    z, c = 2 * torch.randn(T, n, generator=g), 0.2 * torch.randn(n, generator=g)
+    _same(cuda_kernels, z, c if with_correction else None, top=top, groups=groups, kept=kept, best=best, score=score, normalized=normalized,
+          floor=1e-20, scale=scale)
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+def test_neighbours_and_ties(cuda_kernels, score):
+    """Logits a float32 step apart are told apart, equal ones go by their index; corrections that all but make up for the difference too."""
+    g = torch.Generator().manual_seed(3)
+    base = torch.randn(400, 1, generator=g)
+    steps = torch.randint(0, 3, (400, 64), generator=g)
+    z = base.expand(400, 64).contiguous()
+    for _ in range(2):
+        z = torch.where(steps > 0, torch.nextafter(z, torch.tensor(10.0)), z)
+        steps = steps - 1
+    _same(cuda_kernels, z, None, top=8, groups=8, kept=3, best=2, score=score)
+    # scores whose sum with the correction is the same but for what float32 cannot see
+    z = torch.randn(300, 64, generator=g)
+    z[150:] = z[0]
+    s = torch.sigmoid(z.double()) if score == "sigmoid" else torch.softmax(z.double(), 1)
+    c = (1.0 - s[200]).float()
+    _same(cuda_kernels, z, c, top=8, groups=4, kept=2, best=2, score=score)
+    _same(cuda_kernels, torch.zeros(5, 48), None, top=8, groups=6, kept=2, best=2, score=score)
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("normalized", [True, False])
+def test_rows_that_leave_nothing(cuda_kernels, score, normalized):
+    z = torch.randn(12, 40, generator=torch.Generator().manual_seed(1))
+    z[0] = -math.inf                                       # all masked
+    z[1, :38] = -math.inf                                  # two left, in one group
+    z[2, 5], z[3] = math.nan, math.nan
+    z[4, 7] = math.inf
+    z[5] = torch.finfo(torch.float32).min                  # masked by the type's lowest value
+    z[6, ::2] = torch.finfo(torch.float32).min
+    z[7, 30:] = math.nan
+    for kept, top in ((2, 8), (5, 8), (1, 8), (5, 32)):
+        ids, w = _same(cuda_kernels, z, None, top=top, groups=5, kept=kept, best=2, score=score, normalized=normalized, floor=1e-20)
+        assert bool((ids >= 0).all()) and bool((ids < 40).all())
+        assert all(len(set(row)) == top for row in ids.tolist())
+        assert not bool(w[[0, 1, 5, 6]].isnan().any())
+    c = torch.zeros(40)
+    c[3], c[12], c[20] = math.inf, -math.inf, math.nan
+    _same(cuda_kernels, z[8:], c, top=8, groups=5, kept=3, best=2, score=score, normalized=normalized)
+
+
+def test_slices_and_graph(cuda_kernels):
+    from inferflux_b200.csrc.ops import PartialSum
+    g = torch.Generator().manual_seed(9)
+    parts = torch.randn(4, 33, 256, generator=g).to(DEV)
+    total = ((parts[0] + parts[1]) + parts[2]) + parts[3]
+    c = 0.1 * torch.randn(256, generator=g).to(DEV)
+    kw = dict(top=8, groups=8, kept=4, floor=1e-20, scale=2.5)
+    want = cuda_kernels.moe_route_groups(total, c, **kw)
+    got = cuda_kernels.moe_route_groups(PartialSum(parts, torch.float32), c, **kw)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert cuda_kernels.moe_route_groups(total[:0], c, **kw)[0].shape == (0, 8)
+    graph = torch.cuda.CUDAGraph()
+    static = total.clone()
+    with torch.cuda.graph(graph):
+        out = cuda_kernels.moe_route_groups(static, c, **kw)
+    static.copy_(total.flip(0))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out[0], want[0].flip(0)) and torch.equal(out[1], want[1].flip(0))
+
+
+def test_one_group_is_the_flat_router(cuda_kernels):
+    """With one group, the choice of `moe_route` (where no two scores are near) and its weights but for float32's rounding."""
+    z = 2 * torch.randn(200, 64, generator=torch.Generator().manual_seed(2)).to(DEV)
+    c = 0.1 * torch.randn(64, generator=torch.Generator().manual_seed(4)).to(DEV)
+    ids, w = cuda_kernels.moe_route_groups(z, c, 6, 1, 1, score="sigmoid", normalized=True, floor=1e-6)
+    flat_ids, flat_w = cuda_kernels.moe_route(z, c, 6, kind="sigmoid_normalized", floor=1e-6)
+    assert torch.equal(ids, flat_ids) and torch.allclose(w, flat_w, rtol=2e-6, atol=0)
