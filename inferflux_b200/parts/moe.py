@@ -13,7 +13,9 @@ those alone.  `activation` = `clamped_glu`: an expert has a gate matrix too (sta
 expert's gate rows above its up rows) and, with g = min(W_gate h, limit) and u = clamp(W_up h, -limit, limit),
 makes W_down (g sigmoid(1.702 g) (u + 1)); `silu_glu`: the same stack, W_down (silu(W_gate h) * W_up h), nothing cut.
 `routing` = `sigmoid_normalized`: scores = sigmoid(z), the `top` largest are chosen, and the weights are their scores
-divided by (their sum + `weight_floor`).  `shared`: a feed-forward that every token uses; the block adds its output
+divided by (their sum + `weight_floor`).  `groups` = {"count", "kept", "best"}: the experts lie in `count` equal groups, a token uses experts
+of the `kept` groups alone whose `best` largest score + correction sum to the most (csrc/moe_groups.cu); `routing` may then also be
+`softmax_normalized`, softmax scores that are divided like the sigmoid ones, and `weight_scale` multiplies the weights.  `shared`: a feed-forward that every token uses; the block adds its output
 beside the mixture's (forward then returns the pair).
 """
 from __future__ import annotations
@@ -28,7 +30,7 @@ from .base import FeedForward, WeightBuffers, build_part, register_part
 class MixtureOfExperts(FeedForward):
     """params: hidden_size, expert_size (ff of an expert), num_experts, num_identity (default 0), top,
     activation (`relu2` or `clamped_glu` with `limit`), routing (`softmax_of_all`, the default, or
-    `softmax_of_chosen`), correction (whether a selection bias tensor exists; default True),
+    `softmax_of_chosen`; `sigmoid_normalized`; `softmax_normalized`), weight_floor, groups, weight_scale, shared, correction (whether a selection bias tensor exists; default True),
     names (tensor names of router, correction, and the patterns `gate` / `up` / `down` with {e} for the expert's number)."""
 
     _NAMES = {"router": "router", "correction": "correction", "up": "e{e}.up", "down": "e{e}.down", "gate": "e{e}.gate"}
@@ -53,9 +55,15 @@ class MixtureOfExperts(FeedForward):
         self.glu = None if not self.gated else ((self.limit, self.GLU_SLOPE, 1.0) if self.activation == "clamped_glu"
                                                 else (float("inf"), 1.0, 0.0))
         self.routing = str(p.get("routing", "softmax_of_all"))
-        if self.routing not in ("softmax_of_all", "softmax_of_chosen", "sigmoid_normalized"):
+        if self.routing not in ("softmax_of_all", "softmax_of_chosen", "sigmoid_normalized", "softmax_normalized"):
             raise ValueError(f"moe: unknown routing {self.routing!r}")
         self.weight_floor = float(p.get("weight_floor", 0.0))
+        self.weight_scale = float(p.get("weight_scale", 1.0))
+        # (groups, kept, best) of the router by groups, which also scales and normalises softmax scores; None: the flat router
+        self.groups = None
+        if p.get("groups") is not None or self.weight_scale != 1.0 or self.routing == "softmax_normalized":
+            g = p.get("groups") or {"count": 1, "kept": 1, "best": 1}
+            self.groups = (int(g["count"]), int(g["kept"]), int(g.get("best", 2)))
         self.shared = build_part("ffn", p["shared"]) if p.get("shared") is not None else None
         if self.experts < 0 or self.identity < 0 or self.experts + self.identity < 1:
             raise ValueError("moe: there must be at least one expert")
@@ -63,6 +71,15 @@ class MixtureOfExperts(FeedForward):
             raise ValueError(f"moe: top {self.top} of {self.experts + self.identity} experts")
         if self.experts + self.identity > 1024:
             raise ValueError("moe: more than 1024 router outputs are beyond the kernel")
+        if self.groups is not None:
+            count, kept, best = self.groups
+            outs = self.experts + self.identity
+            if self.routing == "softmax_of_chosen":
+                raise ValueError("moe: a softmax over the chosen alone is not built with groups or a scale")
+            if not (1 <= count <= 32 and outs % count == 0 and 1 <= kept <= count and 1 <= best <= outs // count):
+                raise ValueError(f"moe: {outs} experts in {count} groups, {kept} kept by their best {best}")
+            if self.top > min(32, kept * (outs // count)):
+                raise ValueError(f"moe: top {self.top} of {kept} groups of {outs // count} experts (32 at most)")
         self.has_correction = bool(p.get("correction", True))
         self.names = dict(self._NAMES)
         self.names.update(p.get("names") or {})
@@ -115,6 +132,14 @@ class MixtureOfExperts(FeedForward):
             if both is not None:
                 return both(h, self.w_router, correction, self.top, **kind)
             return k.moe_route(k.linear(h, self.w_router, out_dtype=torch.float32), correction, self.top, **kind)
+        if self.groups is not None:
+            count, kept, best = self.groups
+            z = k.linear(h, self.w_router, out_dtype=torch.float32, allow_partial=True)
+            ids, weights = k.moe_route_groups(z, self.correction if self.has_correction else None, self.top, count, kept, best=best,
+                                              score="sigmoid" if self.routing == "sigmoid_normalized" else "softmax",
+                                              normalized=self.routing != "softmax_of_all", floor=self.weight_floor, scale=self.weight_scale)
+            y = k.moe_experts(h, self.w_up, self.w_down, ids, weights, self.experts, ctx.dtype, glu=self.glu)
+            return y if self.shared is None else (y, self.shared.forward(h, ctx))
         if self.routing == "sigmoid_normalized":
             ids, weights = choose(self.correction if self.has_correction else None, kind="sigmoid_normalized", floor=self.weight_floor)
             y = k.moe_experts(h, self.w_up, self.w_down, ids, weights, self.experts, ctx.dtype, glu=self.glu)

@@ -96,3 +96,46 @@ def test_entry_points_refuse():
         return lib.ifx_moe_route_groups(z, splits, n, p, p, T, n_, groups, kept, best, top, 0, 1, f(0), f(1), n)
     assert route(splits=0) == route(T=-1) == route(groups=5) == route(kept=0) == route(kept=9) == route(best=9) == route(top=0) == route(z=n) == -1
     assert route(top=33, kept=8) == route(n_=2048) == route(groups=64, kept=8, best=1) == -4 and route(T=0) == 0
+
+
+# ------------------------------------------------------------------------- a model of such layers, on the plain kernels
+LENS = [40, 33, 3, 61, 97, 1]
+
+
+@pytest.mark.parametrize("which", ["groups", "softmax"])
+@pytest.mark.parametrize("cutting", ["whole", "tail", "portions", "mixed"])
+def test_layers_through_the_step_function(which, cutting):
+    """The selective mixer and experts by groups in a model of their own, cut into steps in every way: the host's side of both parts."""
+    import helpers
+    import selective_models as sm
+    from inferflux_b200.engine import ModelRunner
+    from plain.plain_kernels import PlainKernels
+    model, W = sm.made(which, F32, "cpu")
+    reqs = {f"r{i}": helpers.random_tokens(sm.V, n, 400 + i) for i, n in enumerate(LENS)}
+    want = {r: sm.logits(which, W, toks).numpy() for r, toks in reqs.items()}
+    steps = {"whole": helpers.trace_whole, "tail": helpers.trace_tail, "portions": helpers.trace_portions,
+             "mixed": lambda r: helpers.trace_mixed(r, 256)}[cutting](reqs)
+    runner = ModelRunner(model, PlainKernels(wide=True), page_size=sm.PAGE, num_pages=256 // sm.PAGE, max_seqs=4, max_seq_len=512)
+    got = helpers.collect(steps, helpers.run_steps_in_process(runner, steps), sm.V)
+    bad = helpers.first_bad(got, want, 2e-4)
+    assert bad is None, f"first wrong row (request, position, diff): {bad}"
+
+
+@pytest.mark.parametrize("changes,words", [
+    ({"groups": {"count": 3, "kept": 1, "best": 1}}, "16 experts in 3 groups"), ({"groups": {"count": 4, "kept": 5, "best": 1}}, "5 kept"),
+    ({"groups": {"count": 4, "kept": 1, "best": 5}}, "best 5"), ({"groups": {"count": 4, "kept": 1, "best": 2}, "top": 5}, "top 5"),
+    ({"routing": "softmax_of_chosen", "groups": {"count": 4, "kept": 2, "best": 2}}, "chosen alone"), ({"routing": "other"}, "unknown routing")])
+def test_parts_refuse(changes, words):
+    from inferflux_b200.config import PartSpec
+    from inferflux_b200.parts import build_part
+    p = {"hidden_size": 8, "expert_size": 4, "num_experts": 16, "top": 4, "routing": "sigmoid_normalized", **changes}
+    with pytest.raises(ValueError, match=words):
+        build_part("ffn", PartSpec("moe", p))
+
+
+@pytest.mark.parametrize("changes", [{"state_dim": 129}, {"state_dim": 0}, {"conv_taps": 17}, {"step_rank": 9000}, {"inner_size": -1}])
+def test_mixer_refuses(changes):
+    from inferflux_b200.config import PartSpec
+    from inferflux_b200.parts import build_part
+    with pytest.raises(ValueError, match="selective_state_space"):
+        build_part("mixer", PartSpec("selective_state_space", {"hidden_size": 8, "inner_size": 16, "state_dim": 4, "step_rank": 2, "conv_taps": 4, **changes}))
