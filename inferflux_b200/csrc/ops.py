@@ -185,7 +185,7 @@ class CudaKernels:
                    "ifx_selective_scan", "ifx_selective_inputs", "ifx_moe_route_groups",
                    "ifx_set_shared_carveout", "ifx_set_pdl"),
                   ("ifx_delta_rule_scratch_floats", "ifx_chunk_scan_scratch_floats", "ifx_delta_chunks_scratch_floats",
-                   "ifx_attention_prefill_tcgen05_parts_bytes", "ifx_gemm_f32_split_scratch", "ifx_moe_sorted_scratch",
+                   "ifx_attention_prefill_tcgen05_parts_bytes", "ifx_gemm_f32_split_scratch", "ifx_moe_sorted_scratch", "ifx_selective_scan_scratch",
                    "ifx_sample_scratch_bytes", "ifx_latent_attention_mma_workspace", "ifx_layer_workspace_bytes"))
         # long spans of a bfloat16 run's recurrences by stretches of 64 or 128 tokens (0: token after token, for comparisons)
         self.chunk_scans = os.environ.get("INFERFLUX_B200_CHUNK_SCANS", "1") != "0"
@@ -2250,10 +2250,15 @@ class CudaKernels:
         _on_current_device("selective_scan", x, dt, bc, log_rate, state, z, bias, skip, ctx.cu_seqlens, ctx.req_slot)
         out = torch.empty(T, C, dtype=out_dtype, device=x.device)
         if T and R:
+            longest, room, scratch = int(ctx.max_span), 0, None
+            # spans by stretches, as the other scans: in a bfloat16 run alone, whose sums may depend on how a span was cut into steps
+            if self.chunk_scans and out_dtype is torch.bfloat16 and longest >= self.CHUNK_SCAN_MIN_SPAN:
+                room = self.lib.ifx_selective_scan_scratch(R, longest, C, N)
+                scratch = torch.empty(room, dtype=torch.float32, device=x.device) if room else None
             _check(self.lib.ifx_selective_scan(x, ld_x, _DT[x.dtype], dt, ld_dt, _DT[dt.dtype], bc, ld_bc, z, ld_z, log_rate, bias, skip, state,
                                                max(state.stride(0), C * N), ctx.req_slot, ctx.cu_seqlens, out, _DT[out_dtype], R, T,
-                                               int(ctx.max_span), C, N, _stream()), "selective_scan")
-            self.launches += 1
+                                               longest, C, N, scratch, room, _stream()), "selective_scan")
+            self.launches += 2 if room else 1
         return out
 
     # ---------------------------------------------------------------- sampling

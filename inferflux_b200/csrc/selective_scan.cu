@@ -12,6 +12,8 @@
 // A channel's states are spread over neighbouring lanes, four (or two) a lane.  The sum over n is a tree: neighbouring pairs, pairs of
 // pairs, and so on, the same whatever a lane holds, and every h is one chain of multiply-adds from token to token; so a float32 run's
 // bits do not depend on how a request's tokens are cut into steps.
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace ifx {
@@ -28,6 +30,9 @@ struct SelectiveArgs {
   const int* req_slot; const int* cu_seqlens;
   void* out; int out_dtype;                        // [T, channels]
   int channels, states;
+  int per_block;                                   // channels of a block of the span kernel
+  int stretch, pass; float* ends;                  // spans by stretches: see there (pass 0: whole)
+  int wide;                                        // by 16 bytes (8 for bfloat16 rows): 1 x, 2 dt, 4 z, 8 bc, 16 out, 32 state
 };
 
 __device__ __forceinline__ float load_as_f32(const void* p, long long at, int dtype) {
@@ -42,84 +47,579 @@ __device__ __forceinline__ float exp2_fast(float v) {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-// log(1 + e^v) = max(v, 0) + log(1 + e^-|v|), and log(1 + e) = 2 artanh(s) with s = e / (2 + e) <= 1/3, by artanh's own series
-// s (1 + s^2/3 + s^4/5 + ...): relative to the result, which a logarithm of 1 + e is not where e is small.  The terms left out are below
-// (1/9)^8 / 17 = 1.4e-9.
+__device__ __forceinline__ float rcp_fast(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// log(1 + e^v) = max(v, 0) + log(1 + e^-|v|), and log(1 + e) = 2 artanh(s) with s = e / (2 + e) <= 1/3: relative to the result, which a
+// logarithm of 1 + e is not where e is small.  2 artanh(s) / s as the polynomial of degree four in s^2 whose largest relative error on
+// [0, 1/9] is the least (4e-9, by Remez' exchange).
 __device__ __forceinline__ float softplus_f32(float v) {
   const float e = exp2_fast(-fabsf(v) * kLog2e);
-  const float s = __fdividef(e, 2.0f + e), q = s * s;
-  float p = 1.0f / 15.0f;
-  p = fmaf(p, q, 1.0f / 13.0f);
-  p = fmaf(p, q, 1.0f / 11.0f);
-  p = fmaf(p, q, 1.0f / 9.0f);
-  p = fmaf(p, q, 1.0f / 7.0f);
-  p = fmaf(p, q, 1.0f / 5.0f);
-  p = fmaf(p, q, 1.0f / 3.0f);
-  p = fmaf(p, q, 1.0f);
-  return fmaf(2.0f * s, p, fmaxf(v, 0.0f));
+  const float s = e * rcp_fast(2.0f + e), q = s * s;
+  float p = 0.2817833423614502f;
+  p = fmaf(p, q, 0.27960601449012756f);
+  p = fmaf(p, q, 0.40024909377098083f);
+  p = fmaf(p, q, 0.6666631698608398f);
+  p = fmaf(p, q, 2.0f);
+  return fmaf(s, p, fmaxf(v, 0.0f));
 }
 
-__device__ __forceinline__ float silu_f32(float z) {
-  const float e = exp2_fast(-fabsf(z) * kLog2e);                   // the divisor lies between 1 and 2
-  const float big = __fdividef(1.0f, 1.0f + e);
-  return z * (z >= 0.0f ? big : e * big);
+// z / (1 + e^-z); beyond the exponential's range the divisor is infinite and the quotient 0, its limit
+__device__ __forceinline__ float silu_f32(float z) { return z * rcp_fast(1.0f + exp2_fast(-z * kLog2e)); }
+
+// Two numbers at once: each half is rounded as the scalar operation rounds it.
+__device__ __forceinline__ float2 mul_f32x2(float2 a, float2 b) {
+  float2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(r))
+      : "l"(reinterpret_cast<const unsigned long long&>(a)), "l"(reinterpret_cast<const unsigned long long&>(b)));
+  return r;
+}
+__device__ __forceinline__ float2 fma_f32x2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<unsigned long long&>(r))
+      : "l"(reinterpret_cast<const unsigned long long&>(a)), "l"(reinterpret_cast<const unsigned long long&>(b)),
+        "l"(reinterpret_cast<const unsigned long long&>(c)));
+  return r;
 }
 
-// A token of one lane's states: the step's decay and input go into h, and the lane's part of the sum over n comes back.  `real`: how many of
-// the lane's states there are; the others stay 0 (an infinite x times their zero B would be NaN).
-template <int S, bool PAD>
-__device__ __forceinline__ float selective_token(float (&h)[S], const float (&rate2)[S], float dt, float dtx, const float (&b)[S],
-                                                 const float (&c)[S], int real) {
+// The states of one lane, in pairs.
+template <int S>
+struct LaneStates {
+  float2 v[S / 2];
+  __device__ __forceinline__ void load(const float* p, int real) {
 #pragma unroll
-  for (int j = 0; j < S; ++j) {
-    h[j] = fmaf(exp2_fast(dt * rate2[j]), h[j], dtx * b[j]);
-    if (PAD && j >= real) h[j] = 0.0f;
+    for (int j = 0; j < S / 2; ++j) v[j] = make_float2(2 * j < real ? p[2 * j] : 0.0f, 2 * j + 1 < real ? p[2 * j + 1] : 0.0f);
   }
-  float y = fmaf(c[1], h[1], c[0] * h[0]);
+  __device__ __forceinline__ void load_wide(const float* p) {
+    if constexpr (S == 4) {
+      const float4 f = *reinterpret_cast<const float4*>(p);
+      v[0] = make_float2(f.x, f.y);
+      v[1] = make_float2(f.z, f.w);
+    } else {
+      v[0] = *reinterpret_cast<const float2*>(p);
+    }
+  }
+  __device__ __forceinline__ void store(float* p, int real) const {
 #pragma unroll
-  for (int j = 2; j < S; j += 2) y += fmaf(c[j + 1], h[j + 1], c[j] * h[j]);
-  return y;
+    for (int j = 0; j < S / 2; ++j) {
+      if (2 * j < real) p[2 * j] = v[j].x;
+      if (2 * j + 1 < real) p[2 * j + 1] = v[j].y;
+    }
+  }
+  __device__ __forceinline__ void store_wide(float* p) const {
+    if constexpr (S == 4) *reinterpret_cast<float4*>(p) = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+    else *reinterpret_cast<float2*>(p) = v[0];
+  }
+  // log_rate in, -e^log_rate log2 e out
+  __device__ __forceinline__ void to_rate2() {
+#pragma unroll
+    for (int j = 0; j < S / 2; ++j) v[j] = make_float2(-expf(v[j].x) * kLog2e, -expf(v[j].y) * kLog2e);
+  }
+};
+
+// What a token does to one lane's states of one channel, h <- keep h + take, and what it reads out of them.
+template <int S>
+struct LaneToken {
+  LaneStates<S> keep, take;
+  __device__ __forceinline__ void make(const LaneStates<S>& rate2, float step, float in, const LaneStates<S>& b) {
+#pragma unroll
+    for (int j = 0; j < S / 2; ++j) {
+      keep.v[j] = make_float2(exp2_fast(step * rate2.v[j].x), exp2_fast(step * rate2.v[j].y));
+      take.v[j] = make_float2(in * b.v[j].x, in * b.v[j].y);
+    }
+  }
+  // The lane's part of the sum over n.  `real`: how many of the lane's states there are; the others stay 0 (an infinite x times their
+  // zero B would be NaN).
+  template <bool PAD>
+  __device__ __forceinline__ float go(LaneStates<S>& h, const LaneStates<S>& c, int real) const {
+    float2 sum;
+#pragma unroll
+    for (int j = 0; j < S / 2; ++j) {
+      h.v[j] = fma_f32x2(keep.v[j], h.v[j], take.v[j]);
+      if (PAD) {
+        if (2 * j >= real) h.v[j].x = 0.0f;
+        if (2 * j + 1 >= real) h.v[j].y = 0.0f;
+      }
+      sum = j == 0 ? mul_f32x2(c.v[j], h.v[j]) : fma_f32x2(c.v[j], h.v[j], sum);
+    }
+    return sum.x + sum.y;
+  }
+};
+
+// Four neighbouring channels of a row as they lie in memory.
+struct FourRaw { uint4 v; };
+
+__device__ __forceinline__ FourRaw load_four(const void* p, long long at, int dtype, bool wide, int left) {
+  FourRaw r;
+  r.v = make_uint4(0u, 0u, 0u, 0u);
+  if (dtype == IFX_DT_F32) {
+    const uint32_t* q = static_cast<const uint32_t*>(p) + at;
+    if (wide && left >= 4) return FourRaw{*reinterpret_cast<const uint4*>(q)};
+    if (left > 0) r.v.x = q[0];
+    if (left > 1) r.v.y = q[1];
+    if (left > 2) r.v.z = q[2];
+    if (left > 3) r.v.w = q[3];
+  } else {
+    const unsigned short* q = static_cast<const unsigned short*>(p) + at;
+    if (wide && left >= 4) {
+      const uint2 two = *reinterpret_cast<const uint2*>(q);
+      r.v.x = two.x;
+      r.v.y = two.y;
+      return r;
+    }
+    if (left > 0) r.v.x = q[0];
+    if (left > 1) r.v.x |= (uint32_t)q[1] << 16;
+    if (left > 2) r.v.y = q[2];
+    if (left > 3) r.v.y |= (uint32_t)q[3] << 16;
+  }
+  return r;
 }
 
-// LANES lanes a channel, four states a lane; a block of 128 threads walks one request's tokens.
-template <int LANES, bool PAD>
-__global__ void __launch_bounds__(128) selective_scan_kernel(const SelectiveArgs a) {
-  constexpr int S = 4;
-  const int c = (blockIdx.x * 128 + threadIdx.x) / LANES, part = threadIdx.x % LANES, n0 = part * S, r = blockIdx.y;
-  const bool live = c < a.channels;
-  pdl_launch_dependents();
-  const long long first = a.cu_seqlens[r], last = a.cu_seqlens[r + 1];
-  float* st = a.state + (long long)a.req_slot[r] * a.slot_stride + (long long)c * a.states + n0;
-  float rate2[S], h[S], b[S], cc[S];
+__device__ __forceinline__ float4 four_f32(const FourRaw& r, int dtype) {
+  if (dtype == IFX_DT_F32) return make_float4(__uint_as_float(r.v.x), __uint_as_float(r.v.y), __uint_as_float(r.v.z), __uint_as_float(r.v.w));
+  return make_float4(__uint_as_float(r.v.x << 16), __uint_as_float(r.v.x & 0xffff0000u), __uint_as_float(r.v.y << 16),
+                     __uint_as_float(r.v.y & 0xffff0000u));
+}
+
+__device__ __forceinline__ void store_four(void* p, long long at, int dtype, bool wide, int left, const float (&y)[4]) {
+  if (dtype == IFX_DT_F32) {
+    float* q = static_cast<float*>(p) + at;
+    if (wide && left >= 4) {
+      *reinterpret_cast<float4*>(q) = make_float4(y[0], y[1], y[2], y[3]);
+    } else {
 #pragma unroll
-  for (int j = 0; j < S; ++j) rate2[j] = live && n0 + j < a.states ? -expf(a.log_rate[(long long)c * a.states + n0 + j]) * kLog2e : 0.0f;
+      for (int i = 0; i < 4; ++i)
+        if (i < left) q[i] = y[i];
+    }
+  } else {
+    __nv_bfloat16* q = static_cast<__nv_bfloat16*>(p) + at;
+    if (wide && left >= 4) {
+      __nv_bfloat162 lo = __floats2bfloat162_rn(y[0], y[1]), hi = __floats2bfloat162_rn(y[2], y[3]);
+      *reinterpret_cast<uint2*>(q) = make_uint2(reinterpret_cast<uint32_t&>(lo), reinterpret_cast<uint32_t&>(hi));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i < left) q[i] = __float2bfloat16_rn(y[i]);
+    }
+  }
+}
+
+// BYTES into shared memory, zeros where there is nothing to copy.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* to, const void* from, bool there) {
+  const uint32_t at = (uint32_t)__cvta_generic_to_shared(to);
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(at), "l"(from), "n"(BYTES), "r"(there ? BYTES : 0) : "memory");
+}
+
+template <int BYTES>
+__device__ __forceinline__ FourRaw read_four(const void* from) {
+  if constexpr (BYTES == 16) return FourRaw{*static_cast<const uint4*>(from)};
+  const uint2 two = *static_cast<const uint2*>(from);
+  return FourRaw{make_uint4(two.x, two.y, 0u, 0u)};
+}
+
+constexpr int kWalkers = 256, kWorkers = 256, kSpanThreads = kWalkers + kWorkers, kStepThreads = 128;
+constexpr int kLaneStates = 4;             // of a channel in a lane
+
+template <int LANES>
+struct SpanTile {
+  static constexpr int kChannels = kWalkers / LANES;                     // of a block
+  static constexpr int kTokens = LANES == 1 ? 8 : LANES == 2 || LANES == 32 ? 16 : 32;
+  static constexpr int kStates = kLaneStates * LANES;                    // with those that fill up
+  static constexpr int kFours = (kTokens * kChannels + 4 * kWorkers - 1) / (4 * kWorkers);       // of a worker and tile
+  static constexpr int kTogether = 4;                                    // tokens of a group
+  // the lanes' sums [lane][token][channel]: a plane a lane, so placed that a warp's stores fall on different banks (up to 8 lanes)
+  static constexpr int kPlane = kTokens * kChannels + (LANES < 8 ? 32 / LANES : 4);
+  // floats of shared memory: steps and sums twice, B and C and what the workers fetch once a stage
+  static constexpr int kStages = 3;                                      // tiles that are under way at once
+  static constexpr int kSteps = 2 * kChannels * kTokens;
+  static constexpr int kBC = 2 * kStates * kTokens;
+  static constexpr int kRows = kWorkers * kFours;                        // fours of an operand and stage
+};
+
+// Bytes of shared memory, with four channels of x, z and of dt in `xb` and `db` bytes.
+template <int LANES>
+constexpr int span_bytes(int xb, int db) {
+  using T = SpanTile<LANES>;
+  return 4 * (2 * T::kSteps + T::kStages * T::kBC + 2 * LANES * T::kPlane) + T::kStages * T::kRows * (2 * xb + db);
+}
+
+// Four channels' sums over their lanes: neighbours first, then pairs of neighbours, and so on.
+template <int LANES>
+__device__ __forceinline__ void lanes_sum(const float* p, int plane, float (&out)[4]) {
+  if constexpr (LANES == 1) {
+    const float4 f = *reinterpret_cast<const float4*>(p);
+    out[0] = f.x; out[1] = f.y; out[2] = f.z; out[3] = f.w;
+  } else {
+    float more[4];
+    lanes_sum<LANES / 2>(p, plane, out);
+    lanes_sum<LANES / 2>(p + LANES / 2 * plane, plane, more);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) out[j] += more[j];
+  }
+}
+
+// The request of a block: by the lengths of their spans, longest first, so that the last blocks to begin are short ones (more than 32: as
+// they come).
+__device__ __forceinline__ int request_by_length(const int* __restrict__ cu_seqlens, int requests, int place) {
+  if (requests < 2 || requests > 32) return place;
+  const int lane = threadIdx.x & 31;
+  const int mine = lane < requests ? cu_seqlens[lane + 1] - cu_seqlens[lane] : -1;
+  int before = 0;
+  for (int r = 0; r < requests; ++r) {
+    const int other = __shfl_sync(0xffffffffu, mine, r);
+    before += other > mine || (other == mine && r < lane);
+  }
+  return __ffs(__ballot_sync(0xffffffffu, lane < requests && before == place)) - 1;
+}
+
+// Spans of tokens.  A block has up to 256 / LANES channels of one request and goes through its tokens in tiles.  Eight warps walk: a thread has
+// four states of a channel, and while one group of tokens goes through them the next group's decays are made and what the one behind needs
+// is read.  Eight other warps fetch (two tiles ahead), make steps and steps times x of the next tile, and of the tile before add up the
+// lanes' sums over n, finish and store.
+//
+// By stretches (what `stretch` and `pass` say): where channels are few, a span's tokens are cut into stretches of `stretch`, a block each.
+// The first pass walks the first stretch as it is, and of the others but the last only what they make of a state of zeros and how much of what was
+// there they leave, which is one exponential of the steps' sum; both go to `ends`, [request][stretch][channels (states + 1)].  The second
+// pass puts every stretch's first state together from those in front of it and walks again.
+//
+// XT, DT: the dtypes of x (and z and out) and of dt where all rows can be read by four channels; -1: as the arguments say.
+template <int LANES, bool PAD, int XT, int DT>
+__global__ void __launch_bounds__(kSpanThreads, 1) selective_span_kernel(const SelectiveArgs a) {
+  using Tile = SpanTile<LANES>;
+  constexpr int S = kLaneStates, CH = Tile::kChannels, TT = Tile::kTokens, NP = Tile::kStates, K = Tile::kFours, G = Tile::kTogether,
+                PLANE = Tile::kPlane, ST = Tile::kStages;
+  constexpr bool KNOWN = XT >= 0;
+  extern __shared__ __align__(16) float span_s[];
+  float2* const step_s = reinterpret_cast<float2*>(span_s);              // [2][TT][CH]: steps, and steps times x
+  float* const bc_s = span_s + 2 * Tile::kSteps;                         // [ST][TT][2 NP]
+  float* const y_s = bc_s + ST * Tile::kBC;                              // [2][LANES][PLANE]
+  const int r = request_by_length(a.cu_seqlens, gridDim.y, blockIdx.y), k_stretch = blockIdx.z + (a.pass == 2);
+  const int c0 = blockIdx.x * a.per_block, channels = min(a.channels, c0 + a.per_block);
+  const int span = a.cu_seqlens[r + 1] - a.cu_seqlens[r];
+  const long long begin = a.pass ? (long long)k_stretch * a.stretch : 0;
+  const long long first = a.cu_seqlens[r] + begin;
+  const bool last = !a.pass || span - begin <= a.stretch;                // nothing of the span lies behind
+  const int n = (int)min((long long)span - begin, a.pass ? (long long)a.stretch : (long long)span);
+  const bool local = a.pass == 1 && k_stretch > 0;                       // what it makes of zeros, without any output
+  const int tiles = local && last ? 0 : (n + TT - 1) / TT;               // (n <= 0: none)
+  float* const ends = a.ends + (long long)r * (gridDim.z + 1) * a.channels * (a.states + 1);   // (a grid has a stretch less than there are)
+  if (threadIdx.x < kWalkers) {                                          // ---- the walk
+    // neighbouring lanes have neighbouring channels and the same states: what they read of B and C is one address
+    const int tid = threadIdx.x, part = tid % 32 / (32 / LANES), mine = tid / 32 * (32 / LANES) + tid % (32 / LANES), c = c0 + mine,
+              real = c < channels ? a.states - part * S : 0;
+    const bool idle = c0 + tid / 32 * (32 / LANES) >= channels;          // a warp without channels
+    LaneStates<S> rate2, h;
+    const long long at_c = (long long)c * a.states + part * S, end_size = (long long)a.channels * (a.states + 1);
+    rate2.load(a.log_rate + at_c, real);
+    rate2.to_rate2();
+    pdl_wait();
+    if (tiles <= 0) return;
+    float* st = a.state + (long long)a.req_slot[r] * a.slot_stride + at_c;
+    if (a.pass == 2) {                                                   // what the stretches in front leave
+      h.load(ends + at_c, real);
+      for (int k = 1; k < k_stretch; ++k) {
+        const float* end = ends + k * end_size;
+        const float steps = c < channels ? end[(long long)a.channels * a.states + c] : 0.0f;
+        LaneStates<S> more;
+        more.load(end + at_c, real);
+#pragma unroll
+        for (int j = 0; j < S / 2; ++j)
+          h.v[j] = fma_f32x2(make_float2(exp2_fast(steps * rate2.v[j].x), exp2_fast(steps * rate2.v[j].y)), h.v[j], more.v[j]);
+      }
+    } else {
+      h.load(st, local ? 0 : real);
+    }
+    float steps_sum = 0.0f;
+    if (PAD) __syncthreads();
+    __syncthreads();                                                     // tile 0 is there
+    for (int i = 0; i < tiles; ++i) {
+      if (idle) {
+        __syncthreads();
+        continue;
+      }
+      const int at = i & 1, groups = (min(TT, n - i * TT) + G - 1) / G;
+      const float2* steps = step_s + at * TT * CH + mine;
+      const float* bc = bc_s + i % ST * (TT * 2 * NP) + part * S;
+      float* sums = y_s + (at * LANES + part) * PLANE + mine;
+      if (local) {
+        for (int g = 0; g < groups; ++g) {
+          float2 step[G];
+          LaneStates<S> b[G];
+          LaneToken<S> token[G];
+#pragma unroll
+          for (int j = 0; j < G; ++j) {
+            step[j] = steps[j * CH];
+            b[j].load_wide(bc + j * 2 * NP);
+          }
+#pragma unroll
+          for (int j = 0; j < G; ++j) token[j].make(rate2, step[j].x, step[j].y, b[j]);
+#pragma unroll
+          for (int j = 0; j < G; ++j) token[j].template go<PAD>(h, b[j], real);
+          float sum = 0.0f;
+#pragma unroll
+          for (int j = 0; j < G; ++j) sum += step[j].x;
+          steps_sum += sum;
+          steps += G * CH;
+          bc += G * 2 * NP;
+        }
+        __syncthreads();
+        continue;
+      }
+      float2 step[G];
+      LaneStates<S> b[G], c_[G];
+      LaneToken<S> next[G];
+      auto read = [&](int j) {                                           // of the group whose decays are made next
+        step[j] = steps[j * CH];
+        b[j].load_wide(bc + j * 2 * NP);
+      };
+      auto ahead = [&]() {
+        steps += G * CH;
+        bc += G * 2 * NP;
+      };
+      // a group goes through the states; `makes`: there is one behind it, `reads`: and one behind that
+      auto go = [&](auto makes, auto reads) {
+        float before = 0.0f;
+#pragma unroll
+        for (int j = 0; j < G; ++j) {
+          const float y = next[j].template go<PAD>(h, c_[j], real);
+          if constexpr (decltype(makes)::value) {
+            next[j].make(rate2, step[j].x, step[j].y, b[j]);
+            c_[j].load_wide(bc + (j - G) * 2 * NP + NP);
+          }
+          if constexpr (decltype(reads)::value) read(j);
+          if (j > 0) sums[(j - 1) * CH] = before;
+          before = y;
+        }
+        sums[(G - 1) * CH] = before;
+        sums += G * CH;
+      };
+      using Yes = std::true_type;
+      using No = std::false_type;
+#pragma unroll
+      for (int j = 0; j < G; ++j) {
+        read(j);
+        c_[j].load_wide(bc + j * 2 * NP + NP);
+      }
+#pragma unroll
+      for (int j = 0; j < G; ++j) next[j].make(rate2, step[j].x, step[j].y, b[j]);
+      ahead();
+      if (groups > 1) {
+#pragma unroll
+        for (int j = 0; j < G; ++j) read(j);
+        ahead();
+#pragma unroll 1
+        for (int g = 2; g < groups; ++g) {
+          go(Yes{}, Yes{});
+          ahead();
+        }
+        go(Yes{}, No{});
+      }
+      go(No{}, No{});
+      __syncthreads();
+    }
+    if (last) {
+      h.store(st, real);
+    } else if (a.pass == 1) {
+      float* end = ends + k_stretch * end_size;
+      h.store(end + at_c, real);
+      if (part == 0 && c < channels) end[(long long)a.channels * a.states + c] = steps_sum;
+    }
+    return;
+  }
+  // ---- the others: four channels of some of a tile's tokens each
+  const int x_dtype = KNOWN ? XT : a.x_dtype, dt_dtype = KNOWN ? DT : a.dt_dtype, out_dtype = KNOWN ? XT : a.out_dtype;
+  const bool wide_out = KNOWN || (a.wide & 16);
+  const int tid = threadIdx.x - kWalkers, f4 = 4 * (tid % (CH / 4)), ft = tid / (CH / 4);
+  // channels of the four that there are (with known rows all or none), and none for threads behind a tile's tokens
+  const int left = ft < TT ? channels - c0 - f4 : 0;
+  constexpr int kStride = kWorkers / (CH / 4);                           // tokens from one of a thread's to the next
+  static_assert(K == 1 || K * kStride == TT, "a tile's tokens are shared out evenly");
+  float4 bias = make_float4(0.0f, 0.0f, 0.0f, 0.0f), skip = bias;
+  if (a.bias) bias = four_f32(load_four(a.bias, c0 + f4, IFX_DT_F32, false, left), IFX_DT_F32);
+  if (a.skip) skip = four_f32(load_four(a.skip, c0 + f4, IFX_DT_F32, false, left), IFX_DT_F32);
+  pdl_wait();
+  if (tiles <= 0) return;
+  if constexpr (PAD) {
+    for (int i = tid; i < ST * TT * 2 * NP; i += kWorkers) bc_s[i] = 0.0f;
+    __syncthreads();
+  }
+  // A thread copies what it will need of a tile into places of its own; only B and C are for all.
+  constexpr int XB = XT == IFX_DT_BF16 ? 8 : 16, DB = DT == IFX_DT_BF16 ? 8 : 16, kStage = K * kWorkers * (2 * XB + DB);
+  char* const stages = reinterpret_cast<char*>(y_s + 2 * LANES * PLANE);        // [ST]: x [K][worker], z, dt
+  auto place = [&](char* stage, int operand, int k) {
+    return stage + (operand == 2 ? (2 * K + k) * kWorkers * XB - k * kWorkers * (XB - DB) + tid * DB : ((operand * K + k) * kWorkers + tid) * XB);
+  };
+  const int x_size = x_dtype == IFX_DT_F32 ? 4 : 2, dt_size = dt_dtype == IFX_DT_F32 ? 4 : 2, out_size = out_dtype == IFX_DT_F32 ? 4 : 2;
+  // the thread's first token of the tile to fetch, or to store, and from one of its tokens to the next
+  const char* from_x = static_cast<const char*>(a.x) + ((first + ft) * a.ld_x + c0 + f4) * x_size;
+  const char* from_z = static_cast<const char*>(a.z) + ((first + ft) * a.ld_z + c0 + f4) * x_size;
+  const char* from_dt = static_cast<const char*>(a.dt) + ((first + ft) * a.ld_dt + c0 + f4) * dt_size;
+  char* to_out = static_cast<char*>(a.out) + ((first + ft) * a.channels + c0 + f4) * out_size;
+  const long long row_x = a.ld_x * x_size, row_z = a.ld_z * x_size, row_dt = a.ld_dt * dt_size, row_out = (long long)a.channels * out_size;
+  const bool gated = a.z != nullptr && !local;
+  auto fetch = [&](int t0, int to) {                                     // one group of copies
+    if (!PAD && (a.wide & 8)) {
+#pragma unroll
+      for (int k = 0; k < (TT * NP / 2 + kWorkers - 1) / kWorkers; ++k) {
+        const int i = tid + k * kWorkers, t = i / (NP / 2), j = i % (NP / 2) * 4;
+        if (t < TT) copy_async<16>(bc_s + to * Tile::kBC + 4 * i, a.bc + (first + min(t0 + t, n - 1)) * a.ld_bc + j, t0 + t < n);
+      }
+    } else {
+      for (int i = tid; i < TT * 2 * a.states; i += kWorkers) {
+        const int t = i / (2 * a.states), j = i % (2 * a.states);
+        copy_async<4>(bc_s + to * Tile::kBC + t * 2 * NP + (j < a.states ? j : NP + j - a.states),
+                      a.bc + (first + min(t0 + t, n - 1)) * a.ld_bc + j, t0 + t < n);
+      }
+    }
+    char* const stage = stages + to * kStage;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if (t0 + ft + k * kStride < n && left > 0) {
+        if constexpr (KNOWN) {
+          copy_async<DB>(place(stage, 2, k), from_dt + k * kStride * row_dt, true);
+          copy_async<XB>(place(stage, 0, k), from_x + k * kStride * row_x, true);
+          if (gated) copy_async<XB>(place(stage, 1, k), from_z + k * kStride * row_z, true);
+        } else {
+          const FourRaw d = load_four(from_dt + k * kStride * row_dt, 0, dt_dtype, a.wide & 2, left);
+          const FourRaw x = load_four(from_x + k * kStride * row_x, 0, x_dtype, a.wide & 1, left);
+          FourRaw z = x;
+          if (gated) z = load_four(from_z + k * kStride * row_z, 0, x_dtype, a.wide & 4, left);
+          *reinterpret_cast<uint4*>(place(stage, 2, k)) = d.v;
+          *reinterpret_cast<uint4*>(place(stage, 0, k)) = x.v;
+          *reinterpret_cast<uint4*>(place(stage, 1, k)) = z.v;
+        }
+      }
+    }
+    from_x += TT * row_x;
+    from_z += TT * row_z;
+    from_dt += TT * row_dt;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  auto make = [&](int t0, int buffer, int at) {
+    char* const stage = stages + at * kStage;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int t = ft + k * kStride;
+      if (left <= 0) continue;
+      const float4 x = four_f32(read_four<XB>(place(stage, 0, k)), x_dtype), raw = four_f32(read_four<DB>(place(stage, 2, k)), dt_dtype);
+      const float4 step = make_float4(softplus_f32(raw.x + bias.x), softplus_f32(raw.y + bias.y), softplus_f32(raw.z + bias.z), softplus_f32(raw.w + bias.w));
+      float4 lo = make_float4(step.x, step.x * x.x, step.y, step.y * x.y), hi = make_float4(step.z, step.z * x.z, step.w, step.w * x.w);
+      if (t0 + t >= n) lo = hi = make_float4(0.0f, 0.0f, 0.0f, 0.0f);    // (a token that is not there changes nothing)
+      float4* to = reinterpret_cast<float4*>(step_s + (buffer * TT + t) * CH + f4);
+      to[0] = lo;
+      to[1] = hi;
+    }
+  };
+#pragma unroll
+  for (int s = 0; s < ST - 1; ++s) fetch(s * TT, s);
+  asm volatile("cp.async.wait_group %0;" ::"n"(ST - 2) : "memory");
+  make(0, 0, 0);
+  __syncthreads();
+  for (int i = 0, stage = 0; i < tiles; ++i) {
+    const int t0 = i * TT, next = stage + 1 == ST ? 0 : stage + 1;
+    fetch(t0 + (ST - 1) * TT, stage == 0 ? ST - 1 : stage - 1);          // where tile i - 1 was, which everybody is through with
+    asm volatile("cp.async.wait_group %0;" ::"n"(ST - 2) : "memory");    // tile i + 1 is there
+    if (i + 1 < tiles) make(t0 + TT, (i + 1) & 1, next);
+    __syncthreads();                                                     // tile i has been walked, tile i + 1 can be
+    if (!local)
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int t = ft + k * kStride;
+      if (t0 + t >= n || left <= 0) continue;
+      const float4 x = four_f32(read_four<XB>(place(stages + stage * kStage, 0, k)), x_dtype);
+      float out[4];
+      lanes_sum<LANES>(y_s + (i & 1) * LANES * PLANE + t * CH + f4, PLANE, out);
+      if (a.skip) {                                                      // (no skip is not one of zero: x may be infinite)
+        out[0] = fmaf(skip.x, x.x, out[0]);
+        out[1] = fmaf(skip.y, x.y, out[1]);
+        out[2] = fmaf(skip.z, x.z, out[2]);
+        out[3] = fmaf(skip.w, x.w, out[3]);
+      }
+      if (gated) {
+        const float4 z = four_f32(read_four<XB>(place(stages + stage * kStage, 1, k)), x_dtype);
+        out[0] *= silu_f32(z.x);
+        out[1] *= silu_f32(z.y);
+        out[2] *= silu_f32(z.z);
+        out[3] *= silu_f32(z.w);
+      }
+      store_four(to_out + k * kStride * row_out, 0, out_dtype, wide_out, left, out);
+    }
+    to_out += TT * row_out;
+    stage = next;
+  }
+}
+
+// One token a request at most: a thread has four states of a channel of `each` requests, whose rates it makes once.
+template <int LANES, bool PAD>
+__global__ void __launch_bounds__(kStepThreads) selective_step_kernel(const SelectiveArgs a, int requests, int each) {
+  constexpr int kAhead = 4, S = kLaneStates;
+  const int c = (blockIdx.x * kStepThreads + threadIdx.x) / LANES, part = threadIdx.x % LANES, real = a.states - part * S;
+  const bool live = c < a.channels, wide = !PAD && (a.wide & 32);
+  const int r0 = blockIdx.y * each, r1 = min(requests, r0 + each);
+  pdl_launch_dependents();
+  LaneStates<S> rate2;
+  rate2.load(a.log_rate + (long long)c * a.states + part * S, live ? real : 0);
+  rate2.to_rate2();
   const float bias = live && a.bias ? a.bias[c] : 0.0f, skip = live && a.skip ? a.skip[c] : 0.0f;
   pdl_wait();
-  if (first >= last) return;
+  for (int r = r0; r < r1; r += kAhead) {
+    LaneStates<S> h[kAhead], b[kAhead], cc[kAhead];
+    float x[kAhead], dt[kAhead], z[kAhead];
+    long long t[kAhead];
+    float* st[kAhead];
 #pragma unroll
-  for (int j = 0; j < S; ++j) h[j] = live && n0 + j < a.states ? st[j] : 0.0f;
-  for (long long t = first; t < last; ++t) {
-    const float x = live ? load_as_f32(a.x, t * a.ld_x + c, a.x_dtype) : 0.0f;
-    const float dt = live ? softplus_f32(load_as_f32(a.dt, t * a.ld_dt + c, a.dt_dtype) + bias) : 0.0f;
-#pragma unroll
-    for (int j = 0; j < S; ++j) {
-      b[j] = n0 + j < a.states ? a.bc[t * a.ld_bc + n0 + j] : 0.0f;
-      cc[j] = n0 + j < a.states ? a.bc[t * a.ld_bc + a.states + n0 + j] : 0.0f;
+    for (int i = 0; i < kAhead; ++i) {
+      t[i] = -1;
+      x[i] = dt[i] = z[i] = 0.0f;
+      const int q = r + i;
+      if (q >= r1) continue;
+      const int at = a.cu_seqlens[q];
+      st[i] = a.state + (long long)a.req_slot[q] * a.slot_stride + (long long)c * a.states + part * S;
+      if (a.cu_seqlens[q + 1] <= at) continue;
+      t[i] = at;
     }
-    float y = selective_token<S, PAD>(h, rate2, dt, dt * x, b, cc, a.states - n0);
 #pragma unroll
-    for (int o = 1; o < LANES; o <<= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
-    if (live && part == 0) {
-      if (a.skip) y = fmaf(skip, x, y);                       // (no skip is not one of zero: x may be infinite)
-      if (a.z) y *= silu_f32(load_as_f32(a.z, t * a.ld_z + c, a.x_dtype));
-      const long long at = t * a.channels + c;
-      if (a.out_dtype == IFX_DT_F32) static_cast<float*>(a.out)[at] = y;
-      else static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(y);
+    for (int i = 0; i < kAhead; ++i) {
+      if (t[i] < 0) continue;
+      if (wide) {
+        if (live) h[i].load_wide(st[i]);
+        else h[i].load(st[i], 0);
+      } else {
+        h[i].load(st[i], live ? real : 0);
+      }
+      b[i].load(a.bc + t[i] * a.ld_bc + part * S, real);
+      cc[i].load(a.bc + t[i] * a.ld_bc + a.states + part * S, real);
+      if (live) {
+        x[i] = load_as_f32(a.x, t[i] * a.ld_x + c, a.x_dtype);
+        dt[i] = load_as_f32(a.dt, t[i] * a.ld_dt + c, a.dt_dtype);
+        if (a.z) z[i] = load_as_f32(a.z, t[i] * a.ld_z + c, a.x_dtype);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (t[i] < 0) continue;                                            // (the same for a whole block)
+      const float step = softplus_f32(dt[i] + bias), in = step * x[i];
+      LaneToken<S> token;
+      token.make(rate2, step, in, b[i]);
+      float y = token.template go<PAD>(h[i], cc[i], real);
+#pragma unroll
+      for (int o = 1; o < LANES; o <<= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+      if (!live) continue;
+      if (wide) h[i].store_wide(st[i]);
+      else h[i].store(st[i], real);
+      if (part == 0) {
+        if (a.skip) y = fmaf(skip, x[i], y);
+        if (a.z) y *= silu_f32(z[i]);
+        const long long at = t[i] * a.channels + c;
+        if (a.out_dtype == IFX_DT_F32) static_cast<float*>(a.out)[at] = y;
+        else static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(y);
+      }
     }
   }
-#pragma unroll
-  for (int j = 0; j < S; ++j)
-    if (live && n0 + j < a.states) st[j] = h[j];
 }
 
 struct SelectiveInputsArgs {
@@ -165,14 +665,79 @@ __global__ void __launch_bounds__(128) selective_inputs_kernel(const SelectiveIn
 
 using namespace ifx;
 
+static int lanes_of(int states) {
+  int lanes = 1;
+  while (lanes * kLaneStates < states) lanes <<= 1;
+  return lanes;
+}
+
+// Into how many stretches the longest span is cut at most (0: spans are walked whole).  Two passes of stretches side by side take 2 / stretches of
+// the walk, and a launch; all blocks of a pass run at once.  us, whole and by stretches, one span: 1,024 channels of 16 states, 4,000 tokens
+// 176 / 59; 300 16.3 / 15.3; 2,048 channels, 2,048 tokens 94 / 59, 500 25.6 / 21.6; 512 channels, 200 tokens 13.2 / 15.1; 4,096 channels (three stretches), 2,048
+// tokens 100 / 97, 512 27.1 / 30.2.
+static int stretches_of(int channels, int states, int requests, int max_span) {
+  const long long per_block = kWalkers / lanes_of(states), blocks = (channels + per_block - 1) / per_block * requests;
+  const long long most = 148 / blocks + 1;
+  return most >= 4 && max_span >= 256 ? (int)most : 0;
+}
+
+template <int LANES, bool PAD>
+static int launch_selective(SelectiveArgs a, int requests, int max_span, int stretches, cudaStream_t stream) {
+  if (max_span == 1) {
+    const int each = requests >= 16 ? 4 : 1;
+    const dim3 grid((unsigned)(((long long)a.channels * LANES + kStepThreads - 1) / kStepThreads), (unsigned)((requests + each - 1) / each));
+    return launch_pdl(selective_step_kernel<LANES, PAD>, grid, dim3(kStepThreads), 0, stream, 1, a, requests, each);
+  }
+  using Tile = SpanTile<LANES>;
+  constexpr int F = IFX_DT_F32, B = IFX_DT_BF16;
+  auto kernel = selective_span_kernel<LANES, PAD, -1, -1>;
+  int bytes = span_bytes<LANES>(16, 16);
+  if ((a.wide & 19) == 19 && (!a.z || (a.wide & 4)) && a.channels % 4 == 0 && a.out_dtype == a.x_dtype) {
+    kernel = a.x_dtype == F ? (a.dt_dtype == F ? selective_span_kernel<LANES, PAD, F, F> : selective_span_kernel<LANES, PAD, F, B>)
+                            : (a.dt_dtype == F ? selective_span_kernel<LANES, PAD, B, F> : selective_span_kernel<LANES, PAD, B, B>);
+    bytes = span_bytes<LANES>(a.x_dtype == F ? 16 : 8, a.dt_dtype == F ? 16 : 8);
+  }
+  static_assert(span_bytes<LANES>(16, 16) <= 227 * 1024, "shared memory of a block");
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return (int)e;
+  const unsigned full = (unsigned)((a.channels + Tile::kChannels - 1) / Tile::kChannels);
+  if (stretches) {
+    a.stretch = ((max_span + stretches - 1) / stretches + Tile::kTokens - 1) / Tile::kTokens * Tile::kTokens;
+    const unsigned count = (unsigned)((max_span + a.stretch - 1) / a.stretch);
+    for (a.pass = 1; a.pass <= 2; ++a.pass) {
+      const int rc = launch_pdl(kernel, dim3(full, (unsigned)requests, count - 1), dim3(kSpanThreads), bytes, stream, 1, a);
+      if (rc) return rc;
+    }
+    return 0;
+  }
+  // One request: no more blocks than the rounds of 148 that full ones take, but with as few channels as that allows (4,096 channels of 16
+  // states, 2,048 tokens: 131 -> 100 us).  With several, whose lengths differ, smaller blocks only take longer in all (700 tokens of three, 2,048 of 32
+  // states: 22.8 -> 39.5).
+  constexpr int kLeast = 32 / LANES > 4 ? 32 / LANES : 4;                // a warp's channels, and a worker's
+  if (requests == 1) {
+    const long long rounds = (full + 147) / 148;
+    while (a.per_block > kLeast && (a.channels + a.per_block - kLeast - 1) / (a.per_block - kLeast) <= rounds * 148) a.per_block -= kLeast;
+  }
+  const unsigned blocks = (unsigned)((a.channels + a.per_block - 1) / a.per_block);
+  return launch_pdl(kernel, dim3(blocks, (unsigned)requests), dim3(kSpanThreads), bytes, stream, 1, a);
+}
+
 static bool known_dtype(int d) { return d == IFX_DT_F32 || d == IFX_DT_BF16; }
 
+// Floats that spans walked by stretches need (0: they are walked whole), for a step of so many requests whose longest span has max_span tokens.
+extern "C" long long ifx_selective_scan_scratch(int num_requests, int max_span, int channels, int states) {
+  if (num_requests <= 0 || num_requests > 65535 || max_span <= 1 || channels <= 0 || states <= 0 || states > 128) return 0;
+  return stretches_of(channels, states, num_requests, max_span) * (long long)num_requests * channels * (states + 1);
+}
+
 // Row strides in elements.  x and z share a dtype; bc: float32 rows of B | C; state: float32, slots slot_stride floats apart.
-// num_tokens: rows of x; cu_seqlens does not go beyond them.  A request without tokens keeps its state.
+// num_tokens: rows of x; cu_seqlens does not go beyond them.  A request without tokens keeps its state.  scratch: with scratch_floats of
+// ifx_selective_scan_scratch long spans may go by stretches, whose sums depend on where a span begins; null and 0: they do not.
 extern "C" int ifx_selective_scan(const void* x, long long ld_x, int x_dtype, const void* dt, long long ld_dt, int dt_dtype, const float* bc,
                                   long long ld_bc, const void* z, long long ld_z, const float* log_rate, const float* bias, const float* skip,
                                   float* state, long long slot_stride, const int* req_slot, const int* cu_seqlens, void* out, int out_dtype,
-                                  int num_requests, int num_tokens, int max_span, int channels, int states, cudaStream_t stream) {
+                                  int num_requests, int num_tokens, int max_span, int channels, int states, float* scratch,
+                                  long long scratch_floats, cudaStream_t stream) {
   if (num_requests < 0 || num_tokens < 0 || max_span < 0 || channels <= 0 || states <= 0) return IFX_E_BADARG;
   if (!known_dtype(x_dtype) || !known_dtype(dt_dtype) || !known_dtype(out_dtype)) return IFX_E_DTYPE;
   if (states > 128 || num_requests > 65535) return IFX_E_TOOBIG;
@@ -180,18 +745,30 @@ extern "C" int ifx_selective_scan(const void* x, long long ld_x, int x_dtype, co
   if (ld_x < channels || ld_dt < channels || (z && ld_z < channels) || ld_bc < 2 * states || slot_stride < (long long)channels * states)
     return IFX_E_BADARG;
   if (!x || !dt || !bc || !log_rate || !state || !req_slot || !cu_seqlens || !out) return IFX_E_BADARG;
-  const SelectiveArgs a{x, ld_x, x_dtype, dt, ld_dt, dt_dtype, bc, ld_bc, z, ld_z, log_rate, bias, skip, state, slot_stride, req_slot, cu_seqlens,
-                        out, out_dtype, channels, states};
-  int lanes = 1;
-  while (lanes * 4 < states) lanes <<= 1;
-  const dim3 grid((unsigned)(((long long)channels * lanes + 127) / 128), num_requests);
-  const bool pad = states != lanes * 4;
-#define IFX_SELECTIVE(L) case L: return launch_pdl(pad ? selective_scan_kernel<L, true> : selective_scan_kernel<L, false>, grid, dim3(128), 0, stream, 1, a)
+  auto four = [](const void* p, long long ld, int dtype) {
+    return (uintptr_t)p % (dtype == IFX_DT_F32 ? 16 : 8) == 0 && ld % 4 == 0;
+  };
+  const int wide = (four(x, ld_x, x_dtype) ? 1 : 0) | (four(dt, ld_dt, dt_dtype) ? 2 : 0) | (z && four(z, ld_z, x_dtype) ? 4 : 0) |
+                   (four(bc, ld_bc, IFX_DT_F32) && states % 4 == 0 ? 8 : 0) | (four(out, channels, out_dtype) ? 16 : 0) |
+                   (four(state, slot_stride, IFX_DT_F32) ? 32 : 0);
+  SelectiveArgs a{x, ld_x, x_dtype, dt, ld_dt, dt_dtype, bc, ld_bc, z, ld_z, log_rate, bias, skip, state, slot_stride, req_slot, cu_seqlens,
+                        out, out_dtype, channels, states, 0, 0, 0, scratch, wide};
+  const int lanes = lanes_of(states);
+  a.per_block = kWalkers / lanes;
+  const int stretches = scratch_floats > 0 ? stretches_of(channels, states, num_requests, max_span) : 0;
+  if (stretches && scratch_floats < stretches * (long long)num_requests * channels * (states + 1)) return IFX_E_BADARG;
+  const bool pad = states != lanes * kLaneStates;
+#define IFX_SELECTIVE(L)                                                                        \
+  return pad ? launch_selective<L, true>(a, num_requests, max_span, stretches, stream)          \
+             : launch_selective<L, false>(a, num_requests, max_span, stretches, stream)
   switch (lanes) {
-    IFX_SELECTIVE(1); IFX_SELECTIVE(2); IFX_SELECTIVE(4); IFX_SELECTIVE(8); IFX_SELECTIVE(16);
-    IFX_SELECTIVE(32);
+    case 1: IFX_SELECTIVE(1);
+    case 2: IFX_SELECTIVE(2);
+    case 4: IFX_SELECTIVE(4);
+    case 8: IFX_SELECTIVE(8);
+    case 16: IFX_SELECTIVE(16);
+    default: IFX_SELECTIVE(32);
   }
-  return IFX_E_BADARG;
 #undef IFX_SELECTIVE
 }
 

@@ -80,7 +80,7 @@ def test_entry_points_refuse():
 
     def scan(x_dtype=0, dt_dtype=0, out_dtype=0, R=1, T=2, span=2, C=8, N=4, ld=8, ld_bc=8, slot=32, x=p, out=p):
         return lib.ifx_selective_scan(x, ll(ld), x_dtype, p, ll(8), dt_dtype, p, ll(ld_bc), n, ll(0), p, n, n, p, ll(slot), p, p, out, out_dtype, R, T, span,
-                                      C, N, n)
+                                      C, N, n, ll(0), n)
     assert scan(C=0) == scan(N=0) == scan(R=-1) == scan(T=-1) == scan(ld=7) == scan(ld_bc=7) == scan(slot=31) == scan(x=n) == scan(out=n) == -1
     assert scan(x_dtype=2) == scan(dt_dtype=7) == scan(out_dtype=-1) == -2
     assert scan(N=129, ld_bc=300, slot=9999) == scan(R=65536) == -4
