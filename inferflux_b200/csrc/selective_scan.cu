@@ -32,12 +32,18 @@ struct SelectiveArgs {
   int channels, states;
   int per_block;                                   // channels of a block of the span kernel
   int stretch, pass; float* ends;                  // spans by stretches: see there (pass 0: whole)
-  int wide;                                        // by 16 bytes (8 for bfloat16 rows): 1 x, 2 dt, 4 z, 8 bc, 16 out, 32 state
+  int wide;                                        // by 16 bytes (8 for bfloat16 rows): 1 x, 2 dt, 4 z, 8 bc, 16 out, 32 state, 64 log_rate
 };
 
 __device__ __forceinline__ float load_as_f32(const void* p, long long at, int dtype) {
   return dtype == IFX_DT_F32 ? static_cast<const float*>(p)[at] : __bfloat162float(static_cast<const __nv_bfloat16*>(p)[at]);
 }
+
+// The same in two steps, so that several reads are under way before the first is looked at.
+__device__ __forceinline__ uint32_t load_raw(const void* p, long long at, int dtype) {
+  return dtype == IFX_DT_F32 ? static_cast<const uint32_t*>(p)[at] : static_cast<const unsigned short*>(p)[at];
+}
+__device__ __forceinline__ float raw_f32(uint32_t raw, int dtype) { return __uint_as_float(dtype == IFX_DT_F32 ? raw : raw << 16); }
 
 __device__ __forceinline__ float exp2_fast(float v) {
   float r;
@@ -553,71 +559,62 @@ __global__ void __launch_bounds__(kSpanThreads, 1) selective_span_kernel(const S
   }
 }
 
-// One token a request at most: a thread has four states of a channel of `each` requests, whose rates it makes once.
-template <int LANES, bool PAD>
-__global__ void __launch_bounds__(kStepThreads) selective_step_kernel(const SelectiveArgs a, int requests, int each) {
-  constexpr int kAhead = 4, S = kLaneStates;
-  const int c = (blockIdx.x * kStepThreads + threadIdx.x) / LANES, part = threadIdx.x % LANES, real = a.states - part * S;
-  const bool live = c < a.channels, wide = !PAD && (a.wide & 32);
-  const int r0 = blockIdx.y * each, r1 = min(requests, r0 + each);
+// One token a request at most: a thread has four states of a channel of Q requests, whose rates it makes once; all its reads are under way
+// before the first is looked at (dtypes that a branch chooses are turned into float32 behind the last of them).  WIDE: states, rates, B
+// and C four at a time.  Bound by the states' way in and out: 64 requests of 7,168 channels of 16 states, 62 MB, 15 us, 4.1 TB/s.
+template <int LANES, bool PAD, bool WIDE, int Q>
+__global__ void __launch_bounds__(kStepThreads) selective_step_kernel(const SelectiveArgs a, int requests) {
+  constexpr int S = kLaneStates, CH = kStepThreads / LANES;
+  const int r0 = blockIdx.y * Q, part = threadIdx.x % LANES, c_mine = blockIdx.x * CH + threadIdx.x / LANES, real = a.states - part * S;
+  const int c = min(c_mine, a.channels - 1);                 // (threads behind the last channel read it, and store nothing)
   pdl_launch_dependents();
-  LaneStates<S> rate2;
-  rate2.load(a.log_rate + (long long)c * a.states + part * S, live ? real : 0);
-  rate2.to_rate2();
-  const float bias = live && a.bias ? a.bias[c] : 0.0f, skip = live && a.skip ? a.skip[c] : 0.0f;
+  LaneStates<S> rate2, h[Q], b[Q], c_[Q];
+  uint32_t x_raw[Q], dt_raw[Q], z_raw[Q];
+  auto get = [&](LaneStates<S>& to, const float* from) {
+    if (WIDE) to.load_wide(from);
+    else to.load(from, real);
+  };
+  get(rate2, a.log_rate + (long long)c * a.states + part * S);
+  const float bias = a.bias ? a.bias[c] : 0.0f, skip = a.skip ? a.skip[c] : 0.0f;
+  int t[Q], behind[Q], slot[Q];
+#pragma unroll
+  for (int q = 0; q < Q; ++q) {
+    const int r = min(r0 + q, requests - 1);
+    t[q] = a.cu_seqlens[r];
+    behind[q] = r0 + q < requests ? a.cu_seqlens[r + 1] : t[q];
+    slot[q] = a.req_slot[r];
+  }
   pdl_wait();
-  for (int r = r0; r < r1; r += kAhead) {
-    LaneStates<S> h[kAhead], b[kAhead], cc[kAhead];
-    float x[kAhead], dt[kAhead], z[kAhead];
-    long long t[kAhead];
-    float* st[kAhead];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      t[i] = -1;
-      x[i] = dt[i] = z[i] = 0.0f;
-      const int q = r + i;
-      if (q >= r1) continue;
-      const int at = a.cu_seqlens[q];
-      st[i] = a.state + (long long)a.req_slot[q] * a.slot_stride + (long long)c * a.states + part * S;
-      if (a.cu_seqlens[q + 1] <= at) continue;
-      t[i] = at;
-    }
+  for (int q = 0; q < Q; ++q) {
+    if (behind[q] <= t[q]) continue;
+    get(h[q], a.state + (long long)slot[q] * a.slot_stride + (long long)c * a.states + part * S);
+    x_raw[q] = load_raw(a.x, t[q] * a.ld_x + c, a.x_dtype);
+    dt_raw[q] = load_raw(a.dt, t[q] * a.ld_dt + c, a.dt_dtype);
+    z_raw[q] = a.z ? load_raw(a.z, t[q] * a.ld_z + c, a.x_dtype) : 0u;
+    get(b[q], a.bc + t[q] * a.ld_bc + part * S);
+    get(c_[q], a.bc + t[q] * a.ld_bc + a.states + part * S);
+  }
+  rate2.to_rate2();
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      if (t[i] < 0) continue;
-      if (wide) {
-        if (live) h[i].load_wide(st[i]);
-        else h[i].load(st[i], 0);
-      } else {
-        h[i].load(st[i], live ? real : 0);
-      }
-      b[i].load(a.bc + t[i] * a.ld_bc + part * S, real);
-      cc[i].load(a.bc + t[i] * a.ld_bc + a.states + part * S, real);
-      if (live) {
-        x[i] = load_as_f32(a.x, t[i] * a.ld_x + c, a.x_dtype);
-        dt[i] = load_as_f32(a.dt, t[i] * a.ld_dt + c, a.dt_dtype);
-        if (a.z) z[i] = load_as_f32(a.z, t[i] * a.ld_z + c, a.x_dtype);
-      }
-    }
+  for (int q = 0; q < Q; ++q) {
+    if (behind[q] <= t[q]) continue;
+    const float x = raw_f32(x_raw[q], a.x_dtype), step = softplus_f32(raw_f32(dt_raw[q], a.dt_dtype) + bias);
+    LaneToken<S> token;
+    token.make(rate2, step, step * x, b[q]);
+    float y = token.template go<PAD>(h[q], c_[q], real);
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      if (t[i] < 0) continue;                                            // (the same for a whole block)
-      const float step = softplus_f32(dt[i] + bias), in = step * x[i];
-      LaneToken<S> token;
-      token.make(rate2, step, in, b[i]);
-      float y = token.template go<PAD>(h[i], cc[i], real);
-#pragma unroll
-      for (int o = 1; o < LANES; o <<= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
-      if (!live) continue;
-      if (wide) h[i].store_wide(st[i]);
-      else h[i].store(st[i], real);
-      if (part == 0) {
-        if (a.skip) y = fmaf(skip, x[i], y);
-        if (a.z) y *= silu_f32(z[i]);
-        const long long at = t[i] * a.channels + c;
-        if (a.out_dtype == IFX_DT_F32) static_cast<float*>(a.out)[at] = y;
-        else static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(y);
-      }
+    for (int o = 1; o < LANES; o <<= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+    if (c_mine >= a.channels) continue;
+    float* st = a.state + (long long)slot[q] * a.slot_stride + (long long)c * a.states + part * S;
+    if (WIDE) h[q].store_wide(st);
+    else h[q].store(st, real);
+    if (part == 0) {
+      if (a.skip) y = fmaf(skip, x, y);
+      if (a.z) y *= silu_f32(raw_f32(z_raw[q], a.x_dtype));
+      const long long at = (long long)t[q] * a.channels + c;
+      if (a.out_dtype == IFX_DT_F32) static_cast<float*>(a.out)[at] = y;
+      else static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(y);
     }
   }
 }
@@ -684,9 +681,15 @@ static int stretches_of(int channels, int states, int requests, int max_span) {
 template <int LANES, bool PAD>
 static int launch_selective(SelectiveArgs a, int requests, int max_span, int stretches, cudaStream_t stream) {
   if (max_span == 1) {
-    const int each = requests >= 16 ? 4 : 1;
-    const dim3 grid((unsigned)(((long long)a.channels * LANES + kStepThreads - 1) / kStepThreads), (unsigned)((requests + each - 1) / each));
-    return launch_pdl(selective_step_kernel<LANES, PAD>, grid, dim3(kStepThreads), 0, stream, 1, a, requests, each);
+    constexpr int kChannels = kStepThreads / LANES;
+    const long long blocks = (a.channels + kChannels - 1) / kChannels;
+    const bool wide = !PAD && (a.wide & 104) == 104;
+    // two requests a thread share its rates; with few requests one, for the shorter way (us, 7,168 channels: 1 request 1.6 / 1.8, 8 3.2 / 3.3, 24
+    // 7.1 / 5.9, 64 18 / 15)
+    const int each = requests >= 12 ? 2 : 1;
+    auto kernel = each == 2 ? (wide ? selective_step_kernel<LANES, PAD, !PAD, 2> : selective_step_kernel<LANES, PAD, false, 2>)
+                            : (wide ? selective_step_kernel<LANES, PAD, !PAD, 1> : selective_step_kernel<LANES, PAD, false, 1>);
+    return launch_pdl(kernel, dim3((unsigned)blocks, (unsigned)((requests + each - 1) / each)), dim3(kStepThreads), 0, stream, 1, a, requests);
   }
   using Tile = SpanTile<LANES>;
   constexpr int F = IFX_DT_F32, B = IFX_DT_BF16;
@@ -750,7 +753,7 @@ extern "C" int ifx_selective_scan(const void* x, long long ld_x, int x_dtype, co
   };
   const int wide = (four(x, ld_x, x_dtype) ? 1 : 0) | (four(dt, ld_dt, dt_dtype) ? 2 : 0) | (z && four(z, ld_z, x_dtype) ? 4 : 0) |
                    (four(bc, ld_bc, IFX_DT_F32) && states % 4 == 0 ? 8 : 0) | (four(out, channels, out_dtype) ? 16 : 0) |
-                   (four(state, slot_stride, IFX_DT_F32) ? 32 : 0);
+                   (four(state, slot_stride, IFX_DT_F32) ? 32 : 0) | ((uintptr_t)log_rate % 16 == 0 ? 64 : 0);
   SelectiveArgs a{x, ld_x, x_dtype, dt, ld_dt, dt_dtype, bc, ld_bc, z, ld_z, log_rate, bias, skip, state, slot_stride, req_slot, cu_seqlens,
                         out, out_dtype, channels, states, 0, 0, 0, scratch, wide};
   const int lanes = lanes_of(states);
