@@ -16,18 +16,19 @@ struct GroupRouteArgs {
   const float* correction;                                 // [n] or null
   int* ids; float* weights;                                // [T, top]
   int T, n, groups, kept, best, top;
+  int lanes, stride;                                       // lanes of a group, and numbers from one group's first to the next one's in shared memory
   int softmax, normalized;
   float floor, scale;
 };
 
-constexpr int kGroupRouteMost = 1024;
+constexpr int kGroupRouteMost = 1024, kGroupRouteWarps = 4;
 
-// Bits ordered as the numbers are; NaN with -inf, and one zero.
+// Bits ordered as the numbers are, of numbers alone (one zero); 0 stands before all of them.
 __device__ __forceinline__ unsigned long long ordered_bits(double v) {
-  if (!(v == v)) v = -INFINITY;
   const unsigned long long u = (unsigned long long)__double_as_longlong(v + 0.0);
   return u >> 63 ? ~u : u | 0x8000000000000000ull;
 }
+__device__ __forceinline__ double number_or_least(double v) { return v == v ? v : -INFINITY; }
 
 __device__ __forceinline__ double warp_sum_f64(double v) {
 #pragma unroll
@@ -35,93 +36,156 @@ __device__ __forceinline__ double warp_sum_f64(double v) {
   return v;
 }
 
-// A warp a token.
-__global__ void __launch_bounds__(128) moe_route_groups_kernel(const GroupRouteArgs a) {
+// A warp a token, whose lane has the experts lane, lane + 32, ... (PER of them at most).  Every v goes to shared memory once, group by group; a group's
+// lanes find its two largest, and the choice goes through registers: the largest high words by one reduction, the low words and then the
+// indices where those are equal.  Bound by the latency of that chain and by the exponentials in float64 (some 25 operations each at half the
+// rate of float32).
+template <int PER>
+__global__ void __launch_bounds__(32 * kGroupRouteWarps) moe_route_groups_kernel(const GroupRouteArgs a) {
   extern __shared__ double v_s[];
   const unsigned all = 0xffffffffu;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long t = (long long)blockIdx.x * 4 + warp;
+  const long long t = (long long)blockIdx.x * kGroupRouteWarps + warp;
+  const int size = a.n / a.groups;
   pdl_launch_dependents();
+  float correction[PER];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) correction[k] = a.correction && lane + 32 * k < a.n ? a.correction[lane + 32 * k] : 0.0f;
   pdl_wait();
   if (t >= a.T) return;
-  double* v = v_s + (size_t)warp * a.n;
-  auto logit = [&](int i) {
-    float s = a.z[t * a.n + i];
-    for (int k = 1; k < a.splits; ++k) s += a.z[(size_t)k * a.split_stride + t * a.n + i];
-    return s;
-  };
+  double* const mine_s = v_s + (size_t)warp * a.groups * a.stride;
+  const float* zr = a.z + t * a.n;
+  float z[PER];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) z[k] = lane + 32 * k < a.n ? zr[lane + 32 * k] : -INFINITY;
+  for (int s = 1; s < a.splits; ++s)
+#pragma unroll
+    for (int k = 0; k < PER; ++k)
+      if (lane + 32 * k < a.n) z[k] += zr[s * a.split_stride + lane + 32 * k];
   double m = 0.0, sum = 1.0;
   if (a.softmax) {
     float most = -INFINITY;
-    for (int i = lane; i < a.n; i += 32) most = fmaxf(most, logit(i));
+#pragma unroll
+    for (int k = 0; k < PER; ++k) most = fmaxf(most, z[k]);
     most = warp_max(most);
-    m = most == -INFINITY ? 0.0 : (double)most;
+    m = most == -INFINITY ? 0.0 : (double)most;              // (nothing to share out: every exponential is 0)
+  }
+  auto weight = [&](float zi) { return a.softmax ? exp((double)zi - m) : 1.0 / (1.0 + exp(-(double)zi)); };
+  double v[PER];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) v[k] = weight(z[k]);         // (behind the last expert: of -inf, 0)
+  if (a.softmax) {
     sum = 0.0;
-    for (int i = lane; i < a.n; i += 32) sum += exp((double)logit(i) - m);
+#pragma unroll
+    for (int k = 0; k < PER; ++k) sum += v[k];
     sum = warp_sum_f64(sum);
+#pragma unroll
+    for (int k = 0; k < PER; ++k) v[k] = sum == 0.0 ? 0.0 : v[k] / sum;
   }
-  auto score = [&](int i) {
-    const double z = (double)logit(i);
-    return a.softmax ? (sum == 0.0 ? 0.0 : exp(z - m) / sum) : 1.0 / (1.0 + exp(-z));
-  };
-  for (int i = lane; i < a.n; i += 32) v[i] = score(i) + (a.correction ? (double)a.correction[i] : 0.0);
-  __syncwarp();
-  // a lane a group: its `best` largest, one after the other in falling order
-  const int size = a.n / a.groups;
-  unsigned long long strength = 0;
-  if (lane < a.groups) {
-    double total = 0.0;
-    unsigned long long before = ~0ull;
-    int before_at = -1;
-    for (int k = 0; k < a.best; ++k) {
-      unsigned long long most = 0;
-      int at = -1;
-      for (int i = 0; i < size; ++i) {
-        const unsigned long long key = ordered_bits(v[lane * size + i]);
-        const bool left = key < before || (key == before && i > before_at);
-        if (left && (at < 0 || key > most)) { most = key; at = i; }
+  unsigned short group[PER];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int i = lane + 32 * k;
+    v[k] = number_or_least(v[k] + (double)correction[k]);
+    group[k] = (unsigned short)(i / size);
+    if (i < a.n && a.groups > 1) mine_s[group[k] * a.stride + i - group[k] * size] = v[k];
+  }
+  // the groups' strengths, group g's in lane g
+  unsigned kept = 1;
+  if (a.groups > 1) {
+    __syncwarp();
+    const int g = lane / a.lanes, sub = lane % a.lanes;
+    const double* members = mine_s + min(g, a.groups - 1) * a.stride;
+    double strength;
+    if (a.best <= 2) {
+      double first = -INFINITY, second = -INFINITY;
+      for (int i = sub; i < size; i += a.lanes) {
+        const double w = members[i];
+        second = fmax(second, fmin(first, w));
+        first = fmax(first, w);
       }
-      total += v[lane * size + at];
-      before = most;
-      before_at = at;
+      for (int o = 1; o < a.lanes; o <<= 1) {
+        const double other = __shfl_xor_sync(all, first, o), next = __shfl_xor_sync(all, second, o);
+        second = fmax(fmin(first, other), fmax(second, next));
+        first = fmax(first, other);
+      }
+      strength = a.best == 1 ? first : first + second;
+    } else {                                                 // one after the other in falling order, by a group's first lane
+      strength = 0.0;
+      unsigned long long before = ~0ull;
+      int before_at = -1;
+      for (int c = 0; c < a.best && sub == 0; ++c) {
+        unsigned long long largest = 0;
+        int at = 0;
+        for (int i = 0; i < size; ++i) {
+          const unsigned long long key = ordered_bits(members[i]);
+          if ((key < before || (key == before && i > before_at)) && key > largest) { largest = key; at = i; }
+        }
+        strength += members[at];
+        before = largest;
+        before_at = at;
+      }
     }
-    strength = ordered_bits(total);
+    strength = __shfl_sync(all, number_or_least(strength), min(lane, a.groups - 1) * a.lanes);
+    int place = 0;
+    for (int j = 0; j < a.groups; ++j) {
+      const double other = __shfl_sync(all, strength, j);
+      place += other > strength || (other == strength && j < lane);
+    }
+    kept = __ballot_sync(all, lane < a.groups && place < a.kept);
   }
-  int place = 0;
-  for (int g = 0; g < a.groups; ++g) {
-    const unsigned long long other = __shfl_sync(all, strength, g);
-    place += other > strength || (other == strength && g < lane);
+  // the choice: a lane's candidates as ordered bits (0: none), the best of them first
+  unsigned hi[PER], lo[PER];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const bool in = lane + 32 * k < a.n && (kept >> group[k] & 1u);
+    const unsigned long long key = in ? ordered_bits(v[k]) : 0ull;
+    hi[k] = (unsigned)(key >> 32);
+    lo[k] = (unsigned)key;
   }
-  const unsigned kept = __ballot_sync(all, lane < a.groups && place < a.kept);
-  // the largest of what is left, `top` times; a lane keeps what it has chosen out by one bit an expert of its own
-  unsigned taken = 0;
-  double mine = 0.0;
+  unsigned best_hi = 0, best_lo = 0;
+  int best_k = 0;
+  auto find = [&]() {
+    best_hi = best_lo = 0;
+    best_k = 0;
+#pragma unroll
+    for (int k = 0; k < PER; ++k)
+      if (hi[k] > best_hi || (hi[k] == best_hi && lo[k] > best_lo)) { best_hi = hi[k]; best_lo = lo[k]; best_k = k; }
+  };
+  find();
   int mine_at = 0;
   for (int c = 0; c < a.top; ++c) {
-    unsigned long long most = 0;
-    int at = 0x7fffffff;
-    for (int i = lane, k = 0; i < a.n; i += 32, ++k) {
-      if (taken >> k & 1u || !(kept >> (i / size) & 1u)) continue;
-      const unsigned long long key = ordered_bits(v[i]);
-      if (at == 0x7fffffff || key > most) { most = key; at = i; }
+    const unsigned most = __reduce_max_sync(all, best_hi);
+    unsigned who = __ballot_sync(all, best_hi == most);
+    if (who & (who - 1)) {                                   // several with this high word
+      const unsigned low = __reduce_max_sync(all, best_hi == most ? best_lo : 0u);
+      const bool in = best_hi == most && best_lo == low;
+      const unsigned least = __reduce_min_sync(all, in ? (unsigned)(lane + 32 * best_k) : 0xffffffffu);
+      who = __ballot_sync(all, in && lane + 32 * best_k == (int)least);
     }
+    const int winner = __ffs(who) - 1, at = __shfl_sync(all, lane + 32 * best_k, winner);
+    if (lane == c) mine_at = at;
+    if (lane == winner) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const unsigned long long om = __shfl_xor_sync(all, most, o);
-      const int oa = __shfl_xor_sync(all, at, o);
-      if (oa != 0x7fffffff && (at == 0x7fffffff || om > most || (om == most && oa < at))) { most = om; at = oa; }
+      for (int k = 0; k < PER; ++k)
+        if (k == best_k) hi[k] = lo[k] = 0;
+      find();
     }
-    if ((at & 31) == lane) taken |= 1u << (at >> 5);
-    if (lane == c) { mine = score(at); mine_at = at; }
   }
-  double total = lane < a.top ? mine : 0.0;
+  double w = 0.0;
+  if (lane < a.top) {
+    float zi = zr[mine_at];
+    for (int s = 1; s < a.splits; ++s) zi += zr[s * a.split_stride + mine_at];
+    w = weight(zi);
+    if (a.softmax) w = sum == 0.0 ? 0.0 : w / sum;
+  }
   if (a.normalized) {
-    total = warp_sum_f64(total) + (double)a.floor;
-    mine = total == 0.0 ? 0.0 : mine / total;
+    const double total = warp_sum_f64(w) + (double)a.floor;
+    w = total == 0.0 ? 0.0 : w / total;
   }
   if (lane < a.top) {
     a.ids[t * a.top + lane] = mine_at;
-    a.weights[t * a.top + lane] = (float)(mine * (double)a.scale);
+    a.weights[t * a.top + lane] = (float)(w * (double)a.scale);
   }
 }
 
@@ -138,6 +202,12 @@ extern "C" int ifx_moe_route_groups(const float* z, int splits, const float* cor
   if (n > kGroupRouteMost || groups > 32 || top > 32) return IFX_E_TOOBIG;
   if (T == 0) return 0;
   if (!z || !ids || !weights) return IFX_E_BADARG;
-  const GroupRouteArgs a{z, splits, (size_t)T * n, correction, ids, weights, T, n, groups, kept, best, top, softmax, normalized, floor, scale};
-  return launch_pdl(moe_route_groups_kernel, dim3((unsigned)((T + 3) / 4)), dim3(128), (size_t)4 * n * sizeof(double), stream, 1, a);
+  GroupRouteArgs a{z, splits, (size_t)T * n, correction, ids, weights, T, n, groups, kept, best, top, 1, n / groups, softmax, normalized, floor, scale};
+  while (2 * a.lanes * groups <= 32) a.lanes *= 2;
+  while (a.stride % 16 != a.lanes % 16) ++a.stride;           // a half warp's reads of 8 bytes fall on different banks
+  const size_t bytes = (size_t)kGroupRouteWarps * groups * a.stride * sizeof(double);       // 32 groups of 32 experts and one: 34 KB; at most 48
+  const dim3 grid((unsigned)((T + kGroupRouteWarps - 1) / kGroupRouteWarps)), block(32 * kGroupRouteWarps);
+  auto kernel = n <= 32 ? moe_route_groups_kernel<1> : n <= 64 ? moe_route_groups_kernel<2> : n <= 128 ? moe_route_groups_kernel<4>
+              : n <= 256 ? moe_route_groups_kernel<8> : n <= 512 ? moe_route_groups_kernel<16> : moe_route_groups_kernel<32>;
+  return launch_pdl(kernel, grid, block, groups > 1 ? bytes : 0, stream, 1, a);
 }
