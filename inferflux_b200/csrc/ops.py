@@ -96,14 +96,25 @@ def _need(cond: bool, msg: str) -> None:
 
 def _on_current_device(what: str, *tensors) -> None:
     """A kernel runs on the current device's stream: a tensor elsewhere is refused before its address is used there."""
-    here = None
     for t in tensors:
-        if t is None:
-            continue
-        if here is None:
-            here = -2 if not t.is_cuda else _RAW_DEVICE() if _RAW_DEVICE is not None else torch.cuda.current_device()
-        if t.get_device() != here:
+        if t is not None and not t.is_cuda:
             raise KernelError(f"{what}: a tensor on {t.device}, which is not the current CUDA device")
+    here = _RAW_DEVICE() if _RAW_DEVICE is not None else torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != here:
+            raise KernelError(f"{what}: a tensor on {t.device}, which is not the current CUDA device")
+
+
+def _device_of(what: str, first: torch.Tensor, *tensors) -> torch.device:
+    """`first`'s device, when it is the current one and all the others (None but for them) are there."""
+    here = first.get_device()                              # (a plain number: a CPU tensor's is -1)
+    for t in tensors:
+        if t is not None and t.get_device() != here:
+            here = -1
+            break
+    if here < 0 or here != (_RAW_DEVICE() if _RAW_DEVICE is not None else torch.cuda.current_device()):
+        _on_current_device(what, first, *tensors)
+    return first.device
 
 
 _I, _F, _P, _LL = ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_longlong       # of the structures below
@@ -1787,19 +1798,18 @@ class CudaKernels:
             raise KernelError(f"moe_route_groups: unknown score {score!r}")
         T, n = z.shape
         src, splits = (z.parts, z.splits) if isinstance(z, PartialSum) else (z, 1)
-        _need(src.dtype == torch.float32 and src.is_contiguous() and (correction is None or (
-            correction.dtype == torch.float32 and correction.is_contiguous() and correction.numel() == n)),
-            "moe_route_groups: contiguous float32 logits and corrections")
-        top, groups, kept, best = int(top), int(groups), int(kept), int(best)
+        if src.dtype is not torch.float32 or not src.is_contiguous() or (correction is not None and (
+                correction.dtype is not torch.float32 or correction.numel() != n or not correction.is_contiguous())):
+            raise KernelError("moe_route_groups: contiguous float32 logits and corrections")
         if not (0 < groups <= 32 and n % groups == 0 and n <= 1024 and 1 <= kept <= groups and 1 <= best <= n // groups
                 and 1 <= top <= min(32, kept * (n // groups))):
             raise KernelError(f"moe_route_groups: {n} experts in {groups} groups, {kept} kept by their best {best}, {top} chosen")
-        _on_current_device("moe_route_groups", src, correction)
-        ids = torch.empty(T, top, dtype=torch.int32, device=src.device)
-        weights = torch.empty(T, top, dtype=torch.float32, device=src.device)
+        device = _device_of("moe_route_groups", src, correction)
+        ids = torch.empty(T, top, dtype=torch.int32, device=device)
+        weights = torch.empty(T, top, dtype=torch.float32, device=device)
         if T:
-            _check(self.lib.ifx_moe_route_groups(src, splits, correction, ids, weights, T, n, groups, kept, best, top, int(score == "softmax"),
-                                                 int(bool(normalized)), float(floor), float(scale), _stream()), "moe_route_groups")
+            _check(self.lib.ifx_moe_route_groups(src, splits, correction, ids, weights, T, n, groups, kept, best, top, 1 if score == "softmax" else 0,
+                                                 1 if normalized else 0, floor, scale, _stream()), "moe_route_groups")
             self.launches += 1
         return ids, weights
 
@@ -2186,36 +2196,26 @@ class CudaKernels:
         """rows [T, >= rank + 2 states] (float32 or bfloat16, rows maybe further apart, or a PartialSum) hold a step's low-rank part, B and C side
         by side: returns (the low-rank part [T, rank] in `out_dtype`, B | C float32 [T, 2 states]).  `norms` = (w_low [rank],
         w_b [states], w_c [states]), float32 or None each: that part over its own root mean square (with `eps`), times its weight."""
-        rank, states = int(rank), int(states)
         T, width = rows.shape
         src, splits = (rows.parts, rows.splits) if isinstance(rows, PartialSum) else (rows, 1)
         w_low, w_b, w_c = (None, None, None) if norms is None else norms
         if not (0 < rank <= 8192 and 0 < states <= self.SELECTIVE_MOST_STATES and width >= rank + 2 * states):
             raise KernelError(f"selective_inputs: a rank of {rank} and {states} states in rows of {width}")
-        _need(src.dtype in _DT and out_dtype in _DT and src.stride(-1) == 1 and (splits == 1 or src.is_contiguous())
-              and src.dtype in (torch.float32, torch.bfloat16), "selective_inputs: float32 or bfloat16 rows with unit column stride")
+        code, low_code, strides = _DT.get(src.dtype), _DT.get(out_dtype), src.stride()
+        if code is None or low_code is None or strides[-1] != 1 or (T > 1 and strides[-2] < width) or (splits > 1 and not src.is_contiguous()):
+            raise KernelError("selective_inputs: float32 or bfloat16 rows with unit column stride, one behind the other")
         for w, n in ((w_low, rank), (w_b, states), (w_c, states)):
-            _need(w is None or (w.dtype == torch.float32 and w.is_contiguous() and w.numel() == n),
-                  "selective_inputs: norm weights are float32 of their part's size")
-        _on_current_device("selective_inputs", src, w_low, w_b, w_c)
-        low = torch.empty(T, rank, dtype=out_dtype, device=src.device)
-        bc = torch.empty(T, 2 * states, dtype=torch.float32, device=src.device)
+            if w is not None and (w.dtype is not torch.float32 or w.numel() != n or not w.is_contiguous()):
+                raise KernelError("selective_inputs: norm weights are float32 of their part's size")
+        device = _device_of("selective_inputs", src, w_low, w_b, w_c)
+        low = torch.empty(T, rank, dtype=out_dtype, device=device)
+        bc = torch.empty(T, 2 * states, dtype=torch.float32, device=device)
         if T:
-            ld = max(int(src.stride(-2)), width)                 # (a single row's stride may be anything)
-            _check(self.lib.ifx_selective_inputs(src, ld, _DT[src.dtype], splits, w_low, w_b, w_c, float(eps), low, _DT[out_dtype], bc, T, rank,
+            # (a single row's stride may be anything)
+            _check(self.lib.ifx_selective_inputs(src, max(strides[-2], width), code, splits, w_low, w_b, w_c, eps, low, low_code, bc, T, rank,
                                                  states, _stream()), "selective_inputs")
             self.launches += 1
         return low, bc
-
-    @staticmethod
-    def _selective_rows(t, T, width, what):
-        """The distance between the rows of a float32 or bfloat16 operand of selective_scan."""
-        if t.dtype not in _DT or t.dim() != 2 or t.shape[0] != T or t.shape[1] != width or (t.stride(1) != 1 and width > 1):
-            raise KernelError(f"selective_scan: {what} must be float32 or bfloat16 [{T}, {width}] with unit column stride")
-        stride = t.stride(0)
-        if T > 1 and stride < width:
-            raise KernelError(f"selective_scan: the rows of {what} overlap")
-        return max(stride, width)
 
     def selective_scan(self, x, dt, bc, log_rate, state, ctx, z=None, bias=None, skip=None, out_dtype=None):
         """Per request and channel c a vector h of `states` float32 numbers, kept in `state` [slots, >= channels states] as [channel, state
@@ -2224,19 +2224,58 @@ class CudaKernels:
         x [T, channels], z (or None: no gate) of its dtype, dt: float32 or bfloat16, rows may be slices of wider rows; bc: float32 [T, 2 states],
         B | C; log_rate: float32 [channels, states]; bias, skip: float32 [channels] or None.  Up to 128 states.  Returns y in
         `out_dtype` (default x's).  The requests of a step are in slots of their own; a request without tokens keeps its state."""
+        if out_dtype is None:
+            out_dtype = x.dtype
+        shape, x_code, dt_code, out_code, cu, slots, R = (x.shape, _DT.get(x.dtype), _DT.get(dt.dtype), _DT.get(out_dtype), ctx.cu_seqlens, ctx.req_slot,
+                                                          ctx.num_requests)
+        # one look at what is usual; what is not is looked at in its turn, for the message
+        f32, i32, C, N = torch.float32, torch.int32, shape[-1], log_rate.shape[-1]
+        ld_x, one_x = x.stride()[-2:] if len(shape) == 2 else (0, 0)
+        ld_dt, one_dt = dt.stride() if dt.shape == shape and one_x else (0, 0)
+        ld_bc, one_bc = bc.stride()[-2:] if bc.dim() == 2 else (0, 0)
+        ld_z, one_z = (0, 1) if z is None else z.stride() if z.shape == shape else (0, 0)
+        slot_stride, one_state = state.stride() if state is not None and state.dim() == 2 else (0, 0)
+        if not (one_x == one_dt == one_z == one_bc == 1 and ld_x >= C and ld_dt >= C and (z is None or (ld_z >= C and z.dtype is x.dtype))
+                and x_code is not None and dt_code is not None and out_code is not None and bc.dtype is f32 and bc.shape == (shape[0], 2 * N)
+                and ld_bc >= 2 * N and 0 < N <= self.SELECTIVE_MOST_STATES and C > 0 and log_rate.shape == (C, N) and log_rate.dtype is f32
+                and log_rate.is_contiguous() and (bias is None or (bias.dtype is f32 and bias.numel() == C and bias.is_contiguous()))
+                and (skip is None or (skip.dtype is f32 and skip.numel() == C and skip.is_contiguous())) and one_state == 1
+                and slot_stride >= C * N and state.dtype is f32 and state.shape[1] >= C * N and cu.dtype is i32 and slots.dtype is i32 and cu.numel() > R and slots.numel() >= R and R <= 65535
+                and cu.is_contiguous() and slots.is_contiguous()):
+            ld_x, ld_dt, ld_z, ld_bc, slot_stride = self._selective_scan_operands(x, dt, bc, log_rate, state, ctx, z, bias, skip, out_dtype)
+        T = shape[0]
+        device = _device_of("selective_scan", x, dt, bc, log_rate, state, z, bias, skip, cu, slots)
+        out = torch.empty(T, C, dtype=out_dtype, device=device)
+        if T and R:
+            longest, room, scratch = ctx.max_span, 0, None
+            # spans by stretches, as the other scans: in a bfloat16 run alone, whose sums may depend on how a span was cut into steps
+            if longest >= self.CHUNK_SCAN_MIN_SPAN and self.chunk_scans and out_dtype is torch.bfloat16:
+                room = self.lib.ifx_selective_scan_scratch(R, longest, C, N)
+                scratch = torch.empty(room, dtype=f32, device=device) if room else None
+            _check(self.lib.ifx_selective_scan(x, ld_x, x_code, dt, ld_dt, dt_code, bc, ld_bc, z, ld_z, log_rate, bias, skip, state,
+                                               slot_stride, slots, cu, out, out_code, R, T, longest, C, N, scratch, room, _stream()),
+                   "selective_scan")
+            self.launches += 2 if room else 1
+        return out
+
+    def _selective_scan_operands(self, x, dt, bc, log_rate, state, ctx, z, bias, skip, out_dtype):
+        """The distances between the rows of x, dt, z, bc and the slots of the state, or what is wrong with an operand of selective_scan."""
         _need(x.dim() == 2 and log_rate.dim() == 2, "selective_scan: rows [T, channels] and rates [channels, states]")
-        T, C = x.shape
-        N = log_rate.shape[1]
-        out_dtype = x.dtype if out_dtype is None else out_dtype
-        ld_x, ld_dt = self._selective_rows(x, T, C, "x"), self._selective_rows(dt, T, C, "dt")
-        ld_z = 0
-        if z is not None:
-            _need(z.dtype == x.dtype, "selective_scan: the gate has x's dtype")
-            ld_z = self._selective_rows(z, T, C, "z")
+        (T, C), N = x.shape, log_rate.shape[1]
         if not 0 < N <= self.SELECTIVE_MOST_STATES or C < 1:
             raise KernelError(f"selective_scan: {C} channels of {N} states")
         _need(bc.dtype == torch.float32, "selective_scan: float32 B and C")
-        ld_bc = self._selective_rows(bc, T, 2 * N, "B | C")
+        distances = []
+        for t, width, what in ((x, C, "x"), (dt, C, "dt"), (z, C, "z"), (bc, 2 * N, "B | C")):
+            if t is None:
+                distances.append(0)
+                continue
+            if t.dtype not in _DT or t.dim() != 2 or tuple(t.shape) != (T, width) or (width > 1 and t.stride(1) != 1):
+                raise KernelError(f"selective_scan: {what} must be float32 or bfloat16 [{T}, {width}] with unit column stride")
+            if T > 1 and t.stride(0) < width:
+                raise KernelError(f"selective_scan: the rows of {what} overlap")
+            distances.append(max(t.stride(0), width))          # (a single row's stride may be anything)
+        _need(z is None or z.dtype == x.dtype, "selective_scan: the gate has x's dtype")
         _need(out_dtype in _DT and log_rate.dtype == torch.float32 and log_rate.is_contiguous() and log_rate.shape[0] == C,
               "selective_scan: float32 rates [channels, states], and y in float32 or bfloat16")
         for vec in (bias, skip):
@@ -2244,22 +2283,11 @@ class CudaKernels:
                   "selective_scan: bias and skip are float32 [channels]")
         _need(state is not None and state.dtype == torch.float32 and state.dim() == 2 and state.stride(1) == 1 and state.shape[1] >= C * N
               and (state.shape[0] == 1 or state.stride(0) >= C * N), "selective_scan: the state does not fit the channels")
-        R = int(ctx.num_requests)
-        _need(ctx.cu_seqlens.dtype == torch.int32 and ctx.req_slot.dtype == torch.int32 and ctx.cu_seqlens.numel() > R
-              and ctx.req_slot.numel() >= R and R <= 65535, "selective_scan: int32 spans and slots of every request (up to 65,535)")
-        _on_current_device("selective_scan", x, dt, bc, log_rate, state, z, bias, skip, ctx.cu_seqlens, ctx.req_slot)
-        out = torch.empty(T, C, dtype=out_dtype, device=x.device)
-        if T and R:
-            longest, room, scratch = int(ctx.max_span), 0, None
-            # spans by stretches, as the other scans: in a bfloat16 run alone, whose sums may depend on how a span was cut into steps
-            if self.chunk_scans and out_dtype is torch.bfloat16 and longest >= self.CHUNK_SCAN_MIN_SPAN:
-                room = self.lib.ifx_selective_scan_scratch(R, longest, C, N)
-                scratch = torch.empty(room, dtype=torch.float32, device=x.device) if room else None
-            _check(self.lib.ifx_selective_scan(x, ld_x, _DT[x.dtype], dt, ld_dt, _DT[dt.dtype], bc, ld_bc, z, ld_z, log_rate, bias, skip, state,
-                                               max(state.stride(0), C * N), ctx.req_slot, ctx.cu_seqlens, out, _DT[out_dtype], R, T,
-                                               longest, C, N, scratch, room, _stream()), "selective_scan")
-            self.launches += 2 if room else 1
-        return out
+        R = ctx.num_requests
+        _need(ctx.cu_seqlens.dtype == torch.int32 and ctx.req_slot.dtype == torch.int32 and ctx.cu_seqlens.numel() > R and ctx.cu_seqlens.is_contiguous()
+              and ctx.req_slot.numel() >= R and ctx.req_slot.is_contiguous() and R <= 65535,
+              "selective_scan: int32 spans and slots of every request (up to 65,535)")
+        return *distances, max(state.stride(0), C * N)
 
     # ---------------------------------------------------------------- sampling
     def argmax(self, logits):
