@@ -36,32 +36,27 @@ __device__ __forceinline__ double warp_sum_f64(double v) {
   return v;
 }
 
-// A warp a token, whose lane has the experts lane, lane + 32, ... (PER of them at most).  Every v goes to shared memory once, group by group; a group's
-// lanes find its two largest, and the choice goes through registers: the largest high words by one reduction, the low words and then the
-// indices where those are equal.  Bound by the latency of that chain and by the exponentials in float64 (some 25 operations each at half the
-// rate of float32).
+__device__ __forceinline__ unsigned ordered_bits(float v) {
+  const unsigned u = __float_as_uint(v + 0.0f);
+  return u >> 31 ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float from_ordered(unsigned key) { return __uint_as_float(key >> 31 ? key & 0x7fffffffu : ~key); }
+
+__device__ __forceinline__ double exact_score(const GroupRouteArgs& a, float z, float m, double sum) {
+  return !a.softmax ? 1.0 / (1.0 + exp(-(double)z)) : sum == 0.0 ? 0.0 : exp((double)z - (double)m) / sum;
+}
+
+// One token by a warp, whose lane has the experts lane, lane + 32, ... (PER of them at most).  z: its logits; group: which group an expert of the
+// lane's is in.  Both return the choice, number c in lane c.
+//
+// In float64: every v goes to shared memory, group by group; a group's lanes find its two largest (more: its first lane does, one after the
+// other), and the choice goes through registers: the largest high words by one reduction, the low words and then the indices where those are
+// equal.
 template <int PER>
-__global__ void __launch_bounds__(32 * kGroupRouteWarps) moe_route_groups_kernel(const GroupRouteArgs a) {
-  extern __shared__ double v_s[];
+__device__ __noinline__ int choose_exactly(const GroupRouteArgs& a, const float (&z)[PER], const float (&correction)[PER],
+                                           const unsigned char (&group)[PER], double* mine_s) {
   const unsigned all = 0xffffffffu;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long t = (long long)blockIdx.x * kGroupRouteWarps + warp;
-  const int size = a.n / a.groups;
-  pdl_launch_dependents();
-  float correction[PER];
-#pragma unroll
-  for (int k = 0; k < PER; ++k) correction[k] = a.correction && lane + 32 * k < a.n ? a.correction[lane + 32 * k] : 0.0f;
-  pdl_wait();
-  if (t >= a.T) return;
-  double* const mine_s = v_s + (size_t)warp * a.groups * a.stride;
-  const float* zr = a.z + t * a.n;
-  float z[PER];
-#pragma unroll
-  for (int k = 0; k < PER; ++k) z[k] = lane + 32 * k < a.n ? zr[lane + 32 * k] : -INFINITY;
-  for (int s = 1; s < a.splits; ++s)
-#pragma unroll
-    for (int k = 0; k < PER; ++k)
-      if (lane + 32 * k < a.n) z[k] += zr[s * a.split_stride + lane + 32 * k];
+  const int lane = threadIdx.x & 31, size = a.n / a.groups;
   double m = 0.0, sum = 1.0;
   if (a.softmax) {
     float most = -INFINITY;
@@ -70,10 +65,9 @@ __global__ void __launch_bounds__(32 * kGroupRouteWarps) moe_route_groups_kernel
     most = warp_max(most);
     m = most == -INFINITY ? 0.0 : (double)most;              // (nothing to share out: every exponential is 0)
   }
-  auto weight = [&](float zi) { return a.softmax ? exp((double)zi - m) : 1.0 / (1.0 + exp(-(double)zi)); };
   double v[PER];
 #pragma unroll
-  for (int k = 0; k < PER; ++k) v[k] = weight(z[k]);         // (behind the last expert: of -inf, 0)
+  for (int k = 0; k < PER; ++k) v[k] = a.softmax ? exp((double)z[k] - m) : 1.0 / (1.0 + exp(-(double)z[k]));     // (behind the last expert 0)
   if (a.softmax) {
     sum = 0.0;
 #pragma unroll
@@ -82,12 +76,10 @@ __global__ void __launch_bounds__(32 * kGroupRouteWarps) moe_route_groups_kernel
 #pragma unroll
     for (int k = 0; k < PER; ++k) v[k] = sum == 0.0 ? 0.0 : v[k] / sum;
   }
-  unsigned short group[PER];
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
     const int i = lane + 32 * k;
     v[k] = number_or_least(v[k] + (double)correction[k]);
-    group[k] = (unsigned short)(i / size);
     if (i < a.n && a.groups > 1) mine_s[group[k] * a.stride + i - group[k] * size] = v[k];
   }
   // the groups' strengths, group g's in lane g
@@ -110,7 +102,7 @@ __global__ void __launch_bounds__(32 * kGroupRouteWarps) moe_route_groups_kernel
         first = fmax(first, other);
       }
       strength = a.best == 1 ? first : first + second;
-    } else {                                                 // one after the other in falling order, by a group's first lane
+    } else {
       strength = 0.0;
       unsigned long long before = ~0ull;
       int before_at = -1;
@@ -126,6 +118,7 @@ __global__ void __launch_bounds__(32 * kGroupRouteWarps) moe_route_groups_kernel
         before_at = at;
       }
     }
+    __syncwarp();
     strength = __shfl_sync(all, number_or_least(strength), min(lane, a.groups - 1) * a.lanes);
     int place = 0;
     for (int j = 0; j < a.groups; ++j) {
@@ -172,12 +165,212 @@ __global__ void __launch_bounds__(32 * kGroupRouteWarps) moe_route_groups_kernel
       find();
     }
   }
+  return mine_at;
+}
+
+// The same in float32: false, and nothing said, where two groups' strengths are nearer than their errors and one of them goes, where two
+// experts of one lane are, or where a number is none; experts of different lanes that are near are told apart in float64 on the spot.
+//
+// A score is off by less than 2^-21: a sigmoid by (0.76 + 0.5 + 2) 2^-23, of which the fast exponential of x, good to 2 + 1.173 |x| steps, makes
+// s (1 - s) (2 + 1.173 |x|) <= 0.76 of them, the sum half a one, and the fast quotient two; a softmax's, by three roundings of what float64 gave.  v is off
+// by half a step of its own more, a strength by its terms' errors and a rounding a sum.
+template <int PER>
+__device__ __forceinline__ bool choose_fast(const GroupRouteArgs& a, const float (&z)[PER], float m, double sum, const float (&score)[PER],
+                                            const float (&correction)[PER], const unsigned char (&group)[PER], float* mine_s, int& chosen) {
+  const unsigned all = 0xffffffffu;
+  const int lane = threadIdx.x & 31, size = a.n / a.groups;
+  float v[PER];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) v[k] = score[k] + correction[k];
+  unsigned kept = 1;
+  if (a.groups > 1) {
+    if (a.best > 4) return false;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const int i = lane + 32 * k;
+      if (i < a.n) mine_s[group[k] * a.stride + i - group[k] * size] = v[k];
+    }
+    __syncwarp();
+    const int g = lane / a.lanes, sub = lane % a.lanes;
+    const float* members = mine_s + min(g, a.groups - 1) * a.stride;
+    float strength, magnitude;                               // of its terms
+    bool numbers = true;                                     // (the largest of a NaN and a number is the number)
+    if (a.best <= 2) {
+      float first = -INFINITY, next = -INFINITY;
+      for (int i = sub; i < size; i += a.lanes) {
+        const float w = members[i];
+        numbers = numbers && w == w;
+        next = fmaxf(next, fminf(first, w));
+        first = fmaxf(first, w);
+      }
+      for (int o = 1; o < a.lanes; o <<= 1) {
+        const float other = __shfl_xor_sync(all, first, o);
+        next = fmaxf(fminf(first, other), fmaxf(next, __shfl_xor_sync(all, next, o)));
+        first = fmaxf(first, other);
+      }
+      strength = a.best == 1 ? first : first + next;
+      magnitude = fabsf(first) + (a.best == 1 ? 0.0f : fabsf(next));
+    } else {
+      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      auto insert = [&](float w) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float less = fminf(top[j], w);
+          top[j] = fmaxf(top[j], w);
+          w = less;
+        }
+      };
+      for (int i = sub; i < size; i += a.lanes) {
+        numbers = numbers && members[i] == members[i];
+        insert(members[i]);
+      }
+      for (int o = 1; o < a.lanes; o <<= 1) {
+        float other[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) other[j] = __shfl_xor_sync(all, top[j], o);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) insert(other[j]);
+      }
+      strength = top[0] + top[1] + top[2] + (a.best == 4 ? top[3] : 0.0f);
+      magnitude = fabsf(top[0]) + fabsf(top[1]) + fabsf(top[2]) + (a.best == 4 ? fabsf(top[3]) : 0.0f);
+    }
+    if (!__all_sync(all, numbers)) return false;
+    strength = __shfl_sync(all, strength, min(lane, a.groups - 1) * a.lanes);
+    int place = 0;
+    for (int j = 0; j < a.groups; ++j) place += __shfl_sync(all, strength, j) > strength;
+    kept = __ballot_sync(all, lane < a.groups && place < a.kept);
+    if (a.kept < a.groups) {
+      const bool in = kept >> lane & 1u;
+      const float inside = from_ordered(__reduce_min_sync(all, in ? ordered_bits(strength) : 0xffffffffu));
+      const float outside = from_ordered(__reduce_max_sync(all, lane < a.groups && !in ? ordered_bits(strength) : 0u));
+      const float most = __uint_as_float(__reduce_max_sync(all, __float_as_uint(magnitude)));
+      if (__popc(kept) != a.kept || !(inside - outside > (a.best + 1) * 0x1p-20f + most * 0x1p-20f)) return false;
+    }
+  }
+  // a lane's candidates (0: none) in falling order, each with its number k in the low bits, which the order's last bits give way to
+  constexpr unsigned kLow = PER - 1;
+  unsigned key[PER];
+#pragma unroll
+  for (int k = 0; k < PER; ++k)
+    key[k] = lane + 32 * k < a.n && (kept >> group[k] & 1u) ? (ordered_bits(v[k]) & ~kLow) | (unsigned)k : 0u;
+#pragma unroll
+  for (int length = 2; length <= PER; length *= 2)           // bitonic merges
+#pragma unroll
+    for (int apart_by = length / 2; apart_by > 0; apart_by /= 2)
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int j = apart_by == length / 2 ? i ^ (length - 1) : i ^ apart_by;      // (the first of a merge: mirrored)
+        if (j > i) {
+          const unsigned large = max(key[i], key[j]);
+          key[j] = min(key[i], key[j]);
+          key[i] = large;
+        }
+      }
+  for (int c = 0; c < a.top; ++c) {
+    const float value = from_ordered(__reduce_max_sync(all, key[0]) & ~kLow);
+    if (!(value - value == 0.0f)) return false;              // no number
+    // those that may be the largest: alone, or told apart in float64 where they are in lanes of their own
+    const float near = value - (0x1p-20f + fabsf(value) * (0x1p-20f + PER * 0x1p-22f));
+    const bool in = key[0] != 0 && from_ordered(key[0] & ~kLow) >= near;
+    unsigned who = __ballot_sync(all, in);
+    if (PER > 1 && __any_sync(all, in && key[PER > 1 ? 1 : 0] != 0 && from_ordered(key[PER > 1 ? 1 : 0] & ~kLow) >= near)) return false;
+    const int mine = lane + 32 * (int)(key[0] & kLow);
+    if (who & (who - 1)) {
+      float zi = 0.0f, ci = 0.0f;
+#pragma unroll
+      for (int k = 0; k < PER; ++k)
+        if (k == (int)(key[0] & kLow)) { zi = z[k]; ci = correction[k]; }
+      double most = in ? exact_score(a, zi, m, sum) + (double)ci : -INFINITY;
+      int at = in ? mine : 0x7fffffff;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        const double other = __shfl_xor_sync(all, most, o);
+        const int other_at = __shfl_xor_sync(all, at, o);
+        if (other > most || (other == most && other_at < at)) { most = other; at = other_at; }
+      }
+      who = 1u << (at & 31);
+    }
+    const int winner = __ffs(who) - 1, at = __shfl_sync(all, mine, winner);
+    if (lane == c) chosen = at;
+    if (lane == winner) {
+#pragma unroll
+      for (int k = 0; k + 1 < PER; ++k) key[k] = key[k + 1];
+      key[PER - 1] = 0;
+    }
+  }
+  return true;
+}
+
+// A warp a token.  Bound by the latency of one token's chain (a decode batch) and by the instructions of all (prompts).
+template <int PER>
+__global__ void __launch_bounds__(32 * kGroupRouteWarps) moe_route_groups_kernel(const GroupRouteArgs a) {
+  extern __shared__ double v_s[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long t = (long long)blockIdx.x * kGroupRouteWarps + warp;
+  const int size = a.n / a.groups;
+  pdl_launch_dependents();
+  float correction[PER];
+  unsigned char group[PER];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    correction[k] = a.correction && lane + 32 * k < a.n ? a.correction[lane + 32 * k] : 0.0f;
+  }
+  int quotient = lane / size, rest = lane % size;            // of lane + 32 k, from one k to the next
+  const int step = 32 / size, step_rest = 32 % size;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    group[k] = (unsigned char)quotient;
+    quotient += step;
+    rest += step_rest;
+    if (rest >= size) { rest -= size; ++quotient; }
+  }
+  pdl_wait();
+  if (t >= a.T) return;
+  double* const mine_s = v_s + (size_t)warp * a.groups * a.stride;
+  const float* zr = a.z + t * a.n;
+  float z[PER];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) z[k] = lane + 32 * k < a.n ? zr[lane + 32 * k] : -INFINITY;
+  for (int s = 1; s < a.splits; ++s)
+#pragma unroll
+    for (int k = 0; k < PER; ++k)
+      if (lane + 32 * k < a.n) z[k] += zr[s * a.split_stride + lane + 32 * k];
+  float score[PER], m = 0.0f;
+  double sum = 1.0;                                          // (in float64: every weight is rounded once)
+  if (a.softmax) {
+    m = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) m = fmaxf(m, z[k]);
+    m = warp_max(m);
+    m = m == -INFINITY ? 0.0f : m;                           // (nothing to share out: every exponential is 0)
+    sum = 0.0;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const double e = exp((double)z[k] - (double)m);
+      sum += e;
+      score[k] = (float)e;
+    }
+    sum = warp_sum_f64(sum);
+    const float share = sum == 0.0 ? 0.0f : (float)(1.0 / sum);
+#pragma unroll
+    for (int k = 0; k < PER; ++k) score[k] *= share;
+  } else {
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {                          // (__fdividef: divisors below 2^126)
+      const float s = __fdividef(1.0f, 1.0f + __expf(fminf(-z[k], 80.0f)));
+      score[k] = z[k] == z[k] ? s : z[k];
+    }
+  }
+  int mine_at = 0;
+  if (!choose_fast<PER>(a, z, m, sum, score, correction, group, reinterpret_cast<float*>(mine_s), mine_at)) {
+    __syncwarp();
+    mine_at = choose_exactly<PER>(a, z, correction, group, mine_s);
+  }
   double w = 0.0;
   if (lane < a.top) {
     float zi = zr[mine_at];
     for (int s = 1; s < a.splits; ++s) zi += zr[s * a.split_stride + mine_at];
-    w = weight(zi);
-    if (a.softmax) w = sum == 0.0 ? 0.0 : w / sum;
+    w = exact_score(a, zi, m, sum);
   }
   if (a.normalized) {
     const double total = warp_sum_f64(w) + (double)a.floor;

@@ -103,3 +103,19 @@ def test_one_group_is_the_flat_router(cuda_kernels):
     ids, w = cuda_kernels.moe_route_groups(z, c, 6, 1, 1, score="sigmoid", normalized=True, floor=1e-6)
     flat_ids, flat_w = cuda_kernels.moe_route(z, c, 6, kind="sigmoid_normalized", floor=1e-6)
     assert torch.equal(ids, flat_ids) and torch.allclose(w, flat_w, rtol=2e-6, atol=0)
+
+
+def test_numbers_of_all_sizes(cuda_kernels):
+    """Corrections that dwarf the scores, of both signs in one group, scores at both ends, and many near ones a row: as in 64 bits."""
+    g = torch.Generator().manual_seed(12)
+    z = torch.randn(300, 96, generator=g)
+    big = torch.where(torch.rand(96, generator=g) < 0.5, 1000.0, -1000.0) + 1e-4 * torch.randn(96, generator=g)
+    for score in ("sigmoid", "softmax"):
+        for best in (1, 2, 3, 4, 5):
+            _same(cuda_kernels, z, big, top=8, groups=12, kept=5, best=best, score=score)
+            _same(cuda_kernels, z, 1e-6 * torch.randn(96, generator=g), top=12, groups=12, kept=5, best=best, score=score)
+            _same(cuda_kernels, 1e-6 * z, None, top=16, groups=6, kept=2, best=best, score=score, normalized=False)
+    wide = 25 * torch.randn(400, 512, generator=g)
+    _same(cuda_kernels, wide, None, top=16, groups=8, kept=4, best=2, score="softmax", floor=1e-20)
+    _same(cuda_kernels, wide.clamp(-30, 30), 0.1 * torch.randn(512, generator=g), top=16, groups=8, kept=4, best=2, score="sigmoid")
+    _same(cuda_kernels, torch.randn(64, 1024, generator=g), None, top=32, groups=32, kept=32, best=2, score="sigmoid")
