@@ -15,8 +15,9 @@ struct GroupRouteArgs {
   const float* z; int splits; size_t split_stride;         // [splits, T, n] partial sums, added in split order
   const float* correction;                                 // [n] or null
   int* ids; float* weights;                                // [T, top]
-  int T, n, groups, kept, best, top;
-  int lanes, stride;                                       // lanes of a group, and numbers from one group's first to the next one's in shared memory
+  int T, n, groups, size, kept, best, top;                 // size: experts of a group
+  int lanes, lane_bits, stride;                            // lanes of a group (a power of two), and numbers from one group's first to the next one's
+  unsigned by_size;                                        // in shared memory; expert i is in group i by_size >> 20 (exact: i, n / groups <= 2^10)
   int softmax, normalized;
   float floor, scale;
 };
@@ -56,7 +57,7 @@ template <int PER>
 __device__ __noinline__ int choose_exactly(const GroupRouteArgs& a, const float (&z)[PER], const float (&correction)[PER],
                                            const unsigned char (&group)[PER], double* mine_s) {
   const unsigned all = 0xffffffffu;
-  const int lane = threadIdx.x & 31, size = a.n / a.groups;
+  const int lane = threadIdx.x & 31, size = a.size;
   double m = 0.0, sum = 1.0;
   if (a.softmax) {
     float most = -INFINITY;
@@ -86,7 +87,7 @@ __device__ __noinline__ int choose_exactly(const GroupRouteArgs& a, const float 
   unsigned kept = 1;
   if (a.groups > 1) {
     __syncwarp();
-    const int g = lane / a.lanes, sub = lane % a.lanes;
+    const int g = lane >> a.lane_bits, sub = lane & (a.lanes - 1);
     const double* members = mine_s + min(g, a.groups - 1) * a.stride;
     double strength;
     if (a.best <= 2) {
@@ -178,7 +179,7 @@ template <int PER>
 __device__ __forceinline__ bool choose_fast(const GroupRouteArgs& a, const float (&z)[PER], float m, double sum, const float (&score)[PER],
                                             const float (&correction)[PER], const unsigned char (&group)[PER], float* mine_s, int& chosen) {
   const unsigned all = 0xffffffffu;
-  const int lane = threadIdx.x & 31, size = a.n / a.groups;
+  const int lane = threadIdx.x & 31, size = a.size;
   float v[PER];
 #pragma unroll
   for (int k = 0; k < PER; ++k) v[k] = score[k] + correction[k];
@@ -191,7 +192,7 @@ __device__ __forceinline__ bool choose_fast(const GroupRouteArgs& a, const float
       if (i < a.n) mine_s[group[k] * a.stride + i - group[k] * size] = v[k];
     }
     __syncwarp();
-    const int g = lane / a.lanes, sub = lane % a.lanes;
+    const int g = lane >> a.lane_bits, sub = lane & (a.lanes - 1);
     const float* members = mine_s + min(g, a.groups - 1) * a.stride;
     float strength, magnitude;                               // of its terms
     bool numbers = true;                                     // (the largest of a NaN and a number is the number)
@@ -270,18 +271,17 @@ __device__ __forceinline__ bool choose_fast(const GroupRouteArgs& a, const float
     const float value = from_ordered(__reduce_max_sync(all, key[0]) & ~kLow);
     if (!(value - value == 0.0f)) return false;              // no number
     // those that may be the largest: alone, or told apart in float64 where they are in lanes of their own
-    const float near = value - (0x1p-20f + fabsf(value) * (0x1p-20f + PER * 0x1p-22f));
-    const bool in = key[0] != 0 && from_ordered(key[0] & ~kLow) >= near;
+    const unsigned near = ordered_bits(value - (0x1p-20f + fabsf(value) * (0x1p-20f + PER * 0x1p-22f)));
+    const bool in = key[0] >= near;                          // (truncated keys on one side only: their last bits are in the bound)
     unsigned who = __ballot_sync(all, in);
-    if (PER > 1 && __any_sync(all, in && key[PER > 1 ? 1 : 0] != 0 && from_ordered(key[PER > 1 ? 1 : 0] & ~kLow) >= near)) return false;
-    const int mine = lane + 32 * (int)(key[0] & kLow);
+    if (PER > 1 && __any_sync(all, key[PER > 1 ? 1 : 0] >= near)) return false;
     if (who & (who - 1)) {
       float zi = 0.0f, ci = 0.0f;
 #pragma unroll
       for (int k = 0; k < PER; ++k)
         if (k == (int)(key[0] & kLow)) { zi = z[k]; ci = correction[k]; }
       double most = in ? exact_score(a, zi, m, sum) + (double)ci : -INFINITY;
-      int at = in ? mine : 0x7fffffff;
+      int at = in ? lane + 32 * (int)(key[0] & kLow) : 0x7fffffff;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
         const double other = __shfl_xor_sync(all, most, o);
@@ -290,7 +290,7 @@ __device__ __forceinline__ bool choose_fast(const GroupRouteArgs& a, const float
       }
       who = 1u << (at & 31);
     }
-    const int winner = __ffs(who) - 1, at = __shfl_sync(all, mine, winner);
+    const int winner = __ffs(who) - 1, at = winner + 32 * (int)(__shfl_sync(all, key[0], winner) & kLow);
     if (lane == c) chosen = at;
     if (lane == winner) {
 #pragma unroll
@@ -307,7 +307,6 @@ __global__ void __launch_bounds__(32 * kGroupRouteWarps) moe_route_groups_kernel
   extern __shared__ double v_s[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long t = (long long)blockIdx.x * kGroupRouteWarps + warp;
-  const int size = a.n / a.groups;
   pdl_launch_dependents();
   float correction[PER];
   unsigned char group[PER];
@@ -315,15 +314,8 @@ __global__ void __launch_bounds__(32 * kGroupRouteWarps) moe_route_groups_kernel
   for (int k = 0; k < PER; ++k) {
     correction[k] = a.correction && lane + 32 * k < a.n ? a.correction[lane + 32 * k] : 0.0f;
   }
-  int quotient = lane / size, rest = lane % size;            // of lane + 32 k, from one k to the next
-  const int step = 32 / size, step_rest = 32 % size;
 #pragma unroll
-  for (int k = 0; k < PER; ++k) {
-    group[k] = (unsigned char)quotient;
-    quotient += step;
-    rest += step_rest;
-    if (rest >= size) { rest -= size; ++quotient; }
-  }
+  for (int k = 0; k < PER; ++k) group[k] = (unsigned char)((lane + 32 * k) * a.by_size >> 20);
   pdl_wait();
   if (t >= a.T) return;
   double* const mine_s = v_s + (size_t)warp * a.groups * a.stride;
@@ -395,8 +387,13 @@ extern "C" int ifx_moe_route_groups(const float* z, int splits, const float* cor
   if (n > kGroupRouteMost || groups > 32 || top > 32) return IFX_E_TOOBIG;
   if (T == 0) return 0;
   if (!z || !ids || !weights) return IFX_E_BADARG;
-  GroupRouteArgs a{z, splits, (size_t)T * n, correction, ids, weights, T, n, groups, kept, best, top, 1, n / groups, softmax, normalized, floor, scale};
-  while (2 * a.lanes * groups <= 32) a.lanes *= 2;
+  const int size = n / groups;
+  GroupRouteArgs a{z, splits, (size_t)T * n, correction, ids, weights, T, n, groups, size, kept, best, top, 1, 0, size,
+                   ((1u << 20) + size - 1) / size, softmax, normalized, floor, scale};
+  while (2 * a.lanes * groups <= 32) {
+    a.lanes *= 2;
+    ++a.lane_bits;
+  }
   while (a.stride % 16 != a.lanes % 16) ++a.stride;           // a half warp's reads of 8 bytes fall on different banks
   const size_t bytes = (size_t)kGroupRouteWarps * groups * a.stride * sizeof(double);       // 32 groups of 32 experts and one: 34 KB; at most 48
   const dim3 grid((unsigned)((T + kGroupRouteWarps - 1) / kGroupRouteWarps)), block(32 * kGroupRouteWarps);
