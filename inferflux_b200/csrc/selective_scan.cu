@@ -628,8 +628,71 @@ struct SelectiveInputsArgs {
   int T, rank, states;
 };
 
-// A warp a row, which it keeps in shared memory between the sum of squares and the result.
+// A warp a row: a lane reads columns lane, lane + 32, ... (PER of them at most) before it looks at the first, and all three parts' sums of
+// squares go through one chain of exchanges.  Bound by latency (few rows), then by the rows' way in and out.
+template <int PER>
 __global__ void __launch_bounds__(128) selective_inputs_kernel(const SelectiveInputsArgs a) {
+  const int lane = threadIdx.x & 31, width = a.rank + 2 * a.states, behind_b = a.rank + a.states;
+  const long long t = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  pdl_launch_dependents();
+  const bool normed = a.w_low || a.w_b || a.w_c;
+  float w[PER];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int i = lane + 32 * k;
+    w[k] = 1.0f;
+    if (normed && i < width) {
+      if (i < a.rank) { if (a.w_low) w[k] = a.w_low[i]; }
+      else if (i < behind_b) { if (a.w_b) w[k] = a.w_b[i - a.rank]; }
+      else if (a.w_c) w[k] = a.w_c[i - behind_b];
+    }
+  }
+  pdl_wait();
+  if (t >= a.T) return;
+  float v[PER];
+  uint32_t raw[PER];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) raw[k] = lane + 32 * k < width ? load_raw(a.rows, t * a.ld + lane + 32 * k, a.dtype) : 0u;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) v[k] = raw_f32(raw[k], a.dtype);
+  for (int s = 1; s < a.splits; ++s) {                                   // (in the order of the slices)
+    const float* more = static_cast<const float*>(a.rows) + s * a.split_stride + t * a.ld + lane;
+#pragma unroll
+    for (int k = 0; k < PER; ++k)
+      if (lane + 32 * k < width) v[k] += more[32 * k];
+  }
+  float scale[3] = {1.0f, 1.0f, 1.0f};
+  if (normed) {
+    float sum[3] = {0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const int i = lane + 32 * k;
+      const float q = v[k] * v[k];
+      if (i < a.rank) sum[0] += q;
+      else if (i < behind_b) sum[1] += q;
+      else sum[2] += q;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+      for (int j = 0; j < 3; ++j) sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], o);
+    if (a.w_low) scale[0] = rsqrtf(sum[0] / (float)a.rank + a.eps);
+    if (a.w_b) scale[1] = rsqrtf(sum[1] / (float)a.states + a.eps);
+    if (a.w_c) scale[2] = rsqrtf(sum[2] / (float)a.states + a.eps);
+  }
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int i = lane + 32 * k;
+    if (i >= width) continue;
+    const float y = normed ? v[k] * scale[i < a.rank ? 0 : i < behind_b ? 1 : 2] * w[k] : v[k];
+    if (i >= a.rank) a.bc[t * 2 * a.states + i - a.rank] = y;
+    else if (a.low_dtype == IFX_DT_F32) static_cast<float*>(a.low)[t * a.rank + i] = y;
+    else static_cast<__nv_bfloat16*>(a.low)[t * a.rank + i] = __float2bfloat16_rn(y);
+  }
+}
+
+// Wide rows: a warp keeps one in shared memory between the sum of squares and the result.
+__global__ void __launch_bounds__(128) selective_inputs_wide_kernel(const SelectiveInputsArgs a) {
   extern __shared__ float rows_s[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, width = a.rank + 2 * a.states;
   const long long t = (long long)blockIdx.x * (blockDim.x >> 5) + warp;
@@ -786,6 +849,11 @@ extern "C" int ifx_selective_inputs(const void* rows, long long ld, int dtype, i
   if (!rows || !low || !bc) return IFX_E_BADARG;
   const SelectiveInputsArgs a{rows, ld, dtype, splits, (size_t)T * ld, w_low, w_b, w_c, eps, low, low_dtype, bc, T, rank, states};
   const int width = rank + 2 * states;
+  if (width <= 512) {
+    auto kernel = width <= 64 ? selective_inputs_kernel<2> : width <= 128 ? selective_inputs_kernel<4> : width <= 256 ? selective_inputs_kernel<8>
+                                                                                                                 : selective_inputs_kernel<16>;
+    return launch_pdl(kernel, dim3((unsigned)((T + 3) / 4)), dim3(128), 0, stream, 1, a);
+  }
   const int warps = width <= 3000 ? 4 : 1;                       // of at most 48 KB of rows a block
-  return launch_pdl(selective_inputs_kernel, dim3((unsigned)((T + warps - 1) / warps)), dim3(32 * warps), (size_t)warps * width * 4, stream, 1, a);
+  return launch_pdl(selective_inputs_wide_kernel, dim3((unsigned)((T + warps - 1) / warps)), dim3(32 * warps), (size_t)warps * width * 4, stream, 1, a);
 }
