@@ -9,9 +9,9 @@
 // h is float32, [channels, states] per request at `state + slot * slot_stride`; a new request finds it zeroed.  Steps, decays, states and sums
 // are float32 whatever the rows' dtype; y is rounded once.
 //
-// A channel's states are spread over neighbouring lanes, four (or two) a lane.  The sum over n is a tree: neighbouring pairs, pairs of
-// pairs, and so on, the same whatever a lane holds, and every h is one chain of multiply-adds from token to token; so a float32 run's
-// bits do not depend on how a request's tokens are cut into steps.
+// A channel's states are spread over lanes, four a lane.  A lane adds its terms as (0 and 2) and (1 and 3), the lanes' sums are added as a tree,
+// neighbours first, and every h is one chain of multiply-adds from token to token, whichever kernel walks; so a float32 run's bits do not depend
+// on how a request's tokens are cut into steps.
 #include <type_traits>
 
 #include "common.cuh"
@@ -283,9 +283,15 @@ __device__ __forceinline__ int request_by_length(const int* __restrict__ cu_seql
 }
 
 // Spans of tokens.  A block has up to 256 / LANES channels of one request and goes through its tokens in tiles.  Eight warps walk: a thread has
-// four states of a channel, and while one group of tokens goes through them the next group's decays are made and what the one behind needs
-// is read.  Eight other warps fetch (two tiles ahead), make steps and steps times x of the next tile, and of the tile before add up the
-// lanes' sums over n, finish and store.
+// four states of a channel.  Eight other warps fetch (two tiles ahead), make steps and steps times x of the next tile, and of the tile before add
+// up the lanes' sums over n, finish and store.
+//
+// Bound: the walk.  A token costs a channel as many exponentials as it has states (16 of them a clock and SM: 52 us for 2,048 tokens of 7,168 channels of
+// 16 states, 65 with those of steps and gates); bytes would take 23.  Measured 124 us: a walking warp issues 24 instructions a token, four of which
+// hold its exponential unit for eight clocks each, and two such warps share a scheduler with two that fetch.  Of what was measured on the way (same
+// sizes, us): walk and rows by the same warps 281, walkers apart 260 with two states a lane and 131 with four (shared memory gives a warp 128 bytes a
+// clock, and what a token's B and C cost it is the same for two states as for four); two channels a thread 150, decays four tokens ahead instead of
+// two 131, a quarter of the exponentials by a polynomial 146, twice the workers 131, half of them 142.
 //
 // By stretches (what `stretch` and `pass` say): where channels are few, a span's tokens are cut into stretches of `stretch`, a block each.
 // The first pass walks the first stretch as it is, and of the others but the last only what they make of a state of zeros and how much of what was
@@ -375,56 +381,77 @@ __global__ void __launch_bounds__(kSpanThreads, 1) selective_span_kernel(const S
         __syncthreads();
         continue;
       }
-      float2 step[G];
-      LaneStates<S> b[G], c_[G];
-      LaneToken<S> next[G];
-      auto read = [&](int j) {                                           // of the group whose decays are made next
-        step[j] = steps[j * CH];
-        b[j].load_wide(bc + j * 2 * NP);
-      };
-      auto ahead = [&]() {
-        steps += G * CH;
-        bc += G * 2 * NP;
-      };
-      // a group goes through the states; `makes`: there is one behind it, `reads`: and one behind that
-      auto go = [&](auto makes, auto reads) {
-        float before = 0.0f;
+      // Pairs of tokens: of the one that goes through the states everything is there; of the next one, whose exponentials are made meanwhile, the
+      // arguments; of the one behind it, what it is made of.
+      struct Pair { LaneStates<S> keep[2], take[2], c[2]; } one, two;
+      float2 step[2];
+      LaneStates<S> b[2];
+      auto read = [&](int q) {                                           // pair q from where the pointers are
 #pragma unroll
-        for (int j = 0; j < G; ++j) {
-          const float y = next[j].template go<PAD>(h, c_[j], real);
-          if constexpr (decltype(makes)::value) {
-            next[j].make(rate2, step[j].x, step[j].y, b[j]);
-            c_[j].load_wide(bc + (j - G) * 2 * NP + NP);
-          }
-          if constexpr (decltype(reads)::value) read(j);
-          if (j > 0) sums[(j - 1) * CH] = before;
-          before = y;
+        for (int j = 0; j < 2; ++j) {
+          step[j] = steps[(2 * q + j) * CH];
+          b[j].load_wide(bc + (2 * q + j) * 2 * NP);
         }
-        sums[(G - 1) * CH] = before;
-        sums += G * CH;
+      };
+      auto refill = [&](Pair& p, int q) {                                // from what has been read: arguments in the place of decays
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+          for (int k = 0; k < S / 2; ++k) {
+            p.keep[j].v[k] = make_float2(step[j].x * rate2.v[k].x, step[j].x * rate2.v[k].y);
+            p.take[j].v[k] = make_float2(step[j].y * b[j].v[k].x, step[j].y * b[j].v[k].y);
+          }
+          p.c[j].load_wide(bc + (2 * q + j) * 2 * NP + NP);
+        }
+      };
+      auto exponentials = [&](Pair& p, int j) {
+#pragma unroll
+        for (int k = 0; k < S / 2; ++k) p.keep[j].v[k] = make_float2(exp2_fast(p.keep[j].v[k].x), exp2_fast(p.keep[j].v[k].y));
       };
       using Yes = std::true_type;
       using No = std::false_type;
+      // the pair q goes; `exps`: there is one behind it, `refills`: and one behind that, which takes its place
+      auto go = [&](Pair& p, Pair& behind, int q, auto exps, auto refills) {
+        float y[2];
 #pragma unroll
-      for (int j = 0; j < G; ++j) {
-        read(j);
-        c_[j].load_wide(bc + j * 2 * NP + NP);
-      }
-#pragma unroll
-      for (int j = 0; j < G; ++j) next[j].make(rate2, step[j].x, step[j].y, b[j]);
-      ahead();
-      if (groups > 1) {
-#pragma unroll
-        for (int j = 0; j < G; ++j) read(j);
-        ahead();
-#pragma unroll 1
-        for (int g = 2; g < groups; ++g) {
-          go(Yes{}, Yes{});
-          ahead();
+        for (int j = 0; j < 2; ++j) {
+          LaneToken<S> t{p.keep[j], p.take[j]};
+          if constexpr (decltype(exps)::value) exponentials(behind, j);
+          y[j] = t.template go<PAD>(h, p.c[j], real);
         }
-        go(Yes{}, No{});
+        if constexpr (decltype(refills)::value) {
+          refill(p, q + 2);
+          read(q + 3);                                                   // (behind a tile's last token: not used)
+        }
+        sums[2 * q * CH] = y[0];
+        sums[(2 * q + 1) * CH] = y[1];
+      };
+      int pairs = (min(TT, n - i * TT) + 1) / 2;
+      read(0);
+      refill(one, 0);
+      exponentials(one, 0);
+      exponentials(one, 1);
+      read(1);
+      refill(two, 1);
+      read(2);
+#pragma unroll 1
+      for (; pairs >= 4; pairs -= 2) {
+        go(one, two, 0, Yes{}, Yes{});
+        go(two, one, 1, Yes{}, Yes{});
+        steps += 4 * CH;
+        bc += 4 * 2 * NP;
+        sums += 4 * CH;
       }
-      go(No{}, No{});
+      if (pairs == 3) {
+        go(one, two, 0, Yes{}, Yes{});
+        go(two, one, 1, Yes{}, No{});
+        go(one, two, 2, No{}, No{});
+      } else if (pairs == 2) {
+        go(one, two, 0, Yes{}, No{});
+        go(two, one, 1, No{}, No{});
+      } else {
+        go(one, two, 0, No{}, No{});
+      }
       __syncthreads();
     }
     if (last) {
@@ -467,13 +494,23 @@ __global__ void __launch_bounds__(kSpanThreads, 1) selective_span_kernel(const S
   char* to_out = static_cast<char*>(a.out) + ((first + ft) * a.channels + c0 + f4) * out_size;
   const long long row_x = a.ld_x * x_size, row_z = a.ld_z * x_size, row_dt = a.ld_dt * dt_size, row_out = (long long)a.channels * out_size;
   const bool gated = a.z != nullptr && !local;
+  // B and C by 16 bytes: a worker's pieces of a tile, which lie as in shared memory but for the distance between rows
+  constexpr int kPieces = (TT * NP / 2 + kWorkers - 1) / kWorkers, kPieceRows = kWorkers / (NP / 2) > 0 ? kWorkers / (NP / 2) : 1;
+  static_assert(PAD || kPieces * kWorkers == TT * NP / 2 || kPieces == 1, "pieces are shared out evenly");
+  const int piece_row = tid / (NP / 2), piece_col = tid % (NP / 2) * 4;
+  const float* from_bc = a.bc + (first + piece_row) * a.ld_bc + piece_col;
   auto fetch = [&](int t0, int to) {                                     // one group of copies
+    const bool whole = t0 + TT <= n;
     if (!PAD && (a.wide & 8)) {
+      if (kPieces > 1 || tid < TT * NP / 2) {
+        float* const to_bc = bc_s + to * Tile::kBC + 4 * tid;
 #pragma unroll
-      for (int k = 0; k < (TT * NP / 2 + kWorkers - 1) / kWorkers; ++k) {
-        const int i = tid + k * kWorkers, t = i / (NP / 2), j = i % (NP / 2) * 4;
-        if (t < TT) copy_async<16>(bc_s + to * Tile::kBC + 4 * i, a.bc + (first + min(t0 + t, n - 1)) * a.ld_bc + j, t0 + t < n);
+        for (int k = 0; k < kPieces; ++k) {
+          const bool there = whole || t0 + piece_row + k * kPieceRows < n;
+          copy_async<16>(to_bc + 4 * k * kWorkers, there ? from_bc + k * kPieceRows * a.ld_bc : a.bc, there);
+        }
       }
+      from_bc += TT * a.ld_bc;
     } else {
       for (int i = tid; i < TT * 2 * a.states; i += kWorkers) {
         const int t = i / (2 * a.states), j = i % (2 * a.states);
@@ -481,10 +518,11 @@ __global__ void __launch_bounds__(kSpanThreads, 1) selective_span_kernel(const S
                       a.bc + (first + min(t0 + t, n - 1)) * a.ld_bc + j, t0 + t < n);
       }
     }
-    char* const stage = stages + to * kStage;
+    if (left > 0) {
+      char* const stage = stages + to * kStage;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      if (t0 + ft + k * kStride < n && left > 0) {
+      for (int k = 0; k < K; ++k) {
+        if (!whole && t0 + ft + k * kStride >= n) break;
         if constexpr (KNOWN) {
           copy_async<DB>(place(stage, 2, k), from_dt + k * kStride * row_dt, true);
           copy_async<XB>(place(stage, 0, k), from_x + k * kStride * row_x, true);
@@ -499,26 +537,54 @@ __global__ void __launch_bounds__(kSpanThreads, 1) selective_span_kernel(const S
           *reinterpret_cast<uint4*>(place(stage, 1, k)) = z.v;
         }
       }
+      from_x += TT * row_x;
+      from_z += TT * row_z;
+      from_dt += TT * row_dt;
     }
-    from_x += TT * row_x;
-    from_z += TT * row_z;
-    from_dt += TT * row_dt;
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
   auto make = [&](int t0, int buffer, int at) {
+    if (left <= 0) return;
     char* const stage = stages + at * kStage;
+    float4* const to = reinterpret_cast<float4*>(step_s + (buffer * TT + ft) * CH + f4);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int t = ft + k * kStride;
-      if (left <= 0) continue;
       const float4 x = four_f32(read_four<XB>(place(stage, 0, k)), x_dtype), raw = four_f32(read_four<DB>(place(stage, 2, k)), dt_dtype);
       const float4 step = make_float4(softplus_f32(raw.x + bias.x), softplus_f32(raw.y + bias.y), softplus_f32(raw.z + bias.z), softplus_f32(raw.w + bias.w));
-      float4 lo = make_float4(step.x, step.x * x.x, step.y, step.y * x.y), hi = make_float4(step.z, step.z * x.z, step.w, step.w * x.w);
-      if (t0 + t >= n) lo = hi = make_float4(0.0f, 0.0f, 0.0f, 0.0f);    // (a token that is not there changes nothing)
-      float4* to = reinterpret_cast<float4*>(step_s + (buffer * TT + t) * CH + f4);
-      to[0] = lo;
-      to[1] = hi;
+      to[k * kStride * CH / 2] = make_float4(step.x, step.x * x.x, step.y, step.y * x.y);
+      to[k * kStride * CH / 2 + 1] = make_float4(step.z, step.z * x.z, step.w, step.w * x.w);
     }
+    if (t0 + TT > n)                                                     // a token that is not there changes nothing
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+        if (t0 + ft + k * kStride >= n) to[k * kStride * CH / 2] = to[k * kStride * CH / 2 + 1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  };
+  auto finish = [&](int t0, int buffer, int at) {
+    if (left <= 0) return;
+    char* const stage = stages + at * kStage;
+    const float* const sums = y_s + buffer * LANES * PLANE + ft * CH + f4;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if (t0 + TT > n && t0 + ft + k * kStride >= n) break;
+      const float4 x = four_f32(read_four<XB>(place(stage, 0, k)), x_dtype);
+      float out[4];
+      lanes_sum<LANES>(sums + k * kStride * CH, PLANE, out);
+      if (a.skip) {                                                      // (no skip is not one of zero: x may be infinite)
+        out[0] = fmaf(skip.x, x.x, out[0]);
+        out[1] = fmaf(skip.y, x.y, out[1]);
+        out[2] = fmaf(skip.z, x.z, out[2]);
+        out[3] = fmaf(skip.w, x.w, out[3]);
+      }
+      if (gated) {
+        const float4 z = four_f32(read_four<XB>(place(stage, 1, k)), x_dtype);
+        out[0] *= silu_f32(z.x);
+        out[1] *= silu_f32(z.y);
+        out[2] *= silu_f32(z.z);
+        out[3] *= silu_f32(z.w);
+      }
+      store_four(to_out + k * kStride * row_out, 0, out_dtype, wide_out, KNOWN ? 4 : left, out);
+    }
+    to_out += TT * row_out;
   };
 #pragma unroll
   for (int s = 0; s < ST - 1; ++s) fetch(s * TT, s);
@@ -531,30 +597,7 @@ __global__ void __launch_bounds__(kSpanThreads, 1) selective_span_kernel(const S
     asm volatile("cp.async.wait_group %0;" ::"n"(ST - 2) : "memory");    // tile i + 1 is there
     if (i + 1 < tiles) make(t0 + TT, (i + 1) & 1, next);
     __syncthreads();                                                     // tile i has been walked, tile i + 1 can be
-    if (!local)
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int t = ft + k * kStride;
-      if (t0 + t >= n || left <= 0) continue;
-      const float4 x = four_f32(read_four<XB>(place(stages + stage * kStage, 0, k)), x_dtype);
-      float out[4];
-      lanes_sum<LANES>(y_s + (i & 1) * LANES * PLANE + t * CH + f4, PLANE, out);
-      if (a.skip) {                                                      // (no skip is not one of zero: x may be infinite)
-        out[0] = fmaf(skip.x, x.x, out[0]);
-        out[1] = fmaf(skip.y, x.y, out[1]);
-        out[2] = fmaf(skip.z, x.z, out[2]);
-        out[3] = fmaf(skip.w, x.w, out[3]);
-      }
-      if (gated) {
-        const float4 z = four_f32(read_four<XB>(place(stages + stage * kStage, 1, k)), x_dtype);
-        out[0] *= silu_f32(z.x);
-        out[1] *= silu_f32(z.y);
-        out[2] *= silu_f32(z.z);
-        out[3] *= silu_f32(z.w);
-      }
-      store_four(to_out + k * kStride * row_out, 0, out_dtype, wide_out, left, out);
-    }
-    to_out += TT * row_out;
+    if (!local) finish(t0, i & 1, stage);
     stage = next;
   }
 }
