@@ -213,11 +213,13 @@ __device__ __forceinline__ void store_four(void* p, long long at, int dtype, boo
   }
 }
 
-// BYTES into shared memory, zeros where there is nothing to copy.
+// BYTES into shared memory, zeros where there is nothing to copy.  16 bytes pass L1 by: with all but 28 KB of an SM's memory shared, as every kernel
+// here asks for, lines that wait for their data fill it (2,048 tokens of 7,168 channels 141 -> 123 us).
 template <int BYTES>
 __device__ __forceinline__ void copy_async(void* to, const void* from, bool there) {
   const uint32_t at = (uint32_t)__cvta_generic_to_shared(to);
-  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(at), "l"(from), "n"(BYTES), "r"(there ? BYTES : 0) : "memory");
+  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(from), "r"(there ? 16 : 0) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(at), "l"(from), "n"(BYTES), "r"(there ? BYTES : 0) : "memory");
 }
 
 template <int BYTES>
