@@ -43,21 +43,35 @@ __device__ __forceinline__ unsigned ordered_bits(float v) {
 }
 __device__ __forceinline__ float from_ordered(unsigned key) { return __uint_as_float(key >> 31 ? key & 0x7fffffffu : ~key); }
 
+// Logit i of the token whose first lies at `zr`: slices are added in their order.
+__device__ __forceinline__ float logit(const GroupRouteArgs& a, const float* zr, int i) {
+  float z = zr[i];
+  for (int s = 1; s < a.splits; ++s) z += zr[s * a.split_stride + i];
+  return z;
+}
+
 __device__ __forceinline__ double exact_score(const GroupRouteArgs& a, float z, float m, double sum) {
   return !a.softmax ? 1.0 / (1.0 + exp(-(double)z)) : sum == 0.0 ? 0.0 : exp((double)z - (double)m) / sum;
 }
 
-// One token by a warp, whose lane has the experts lane, lane + 32, ... (PER of them at most).  z: its logits; group: which group an expert of the
-// lane's is in.  Both return the choice, number c in lane c.
+// One token by a warp, whose lane has the experts lane, lane + 32, ... (PER of them at most).  zr: its logits.  Both give the choice, number c
+// in lane c.
 //
 // In float64: every v goes to shared memory, group by group; a group's lanes find its two largest (more: its first lane does, one after the
 // other), and the choice goes through registers: the largest high words by one reduction, the low words and then the indices where those are
 // equal.
 template <int PER>
-__device__ __noinline__ int choose_exactly(const GroupRouteArgs& a, const float (&z)[PER], const float (&correction)[PER],
-                                           const unsigned char (&group)[PER], double* mine_s) {
+__device__ __noinline__ int choose_exactly(const GroupRouteArgs& a, const float* zr, double* mine_s) {
   const unsigned all = 0xffffffffu;
   const int lane = threadIdx.x & 31, size = a.size;
+  float z[PER];
+  unsigned char group[PER];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int i = lane + 32 * k;
+    z[k] = i < a.n ? logit(a, zr, i) : -INFINITY;
+    group[k] = (unsigned char)(i * a.by_size >> 20);
+  }
   double m = 0.0, sum = 1.0;
   if (a.softmax) {
     float most = -INFINITY;
@@ -80,7 +94,7 @@ __device__ __noinline__ int choose_exactly(const GroupRouteArgs& a, const float 
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
     const int i = lane + 32 * k;
-    v[k] = number_or_least(v[k] + (double)correction[k]);
+    v[k] = number_or_least(v[k] + (a.correction && i < a.n ? (double)a.correction[i] : 0.0));
     if (i < a.n && a.groups > 1) mine_s[group[k] * a.stride + i - group[k] * size] = v[k];
   }
   // the groups' strengths, group g's in lane g
@@ -176,13 +190,10 @@ __device__ __noinline__ int choose_exactly(const GroupRouteArgs& a, const float 
 // s (1 - s) (2 + 1.173 |x|) <= 0.76 of them, the sum half a one, and the fast quotient two; a softmax's, by three roundings of what float64 gave.  v is off
 // by half a step of its own more, a strength by its terms' errors and a rounding a sum.
 template <int PER>
-__device__ __forceinline__ bool choose_fast(const GroupRouteArgs& a, const float (&z)[PER], float m, double sum, const float (&score)[PER],
-                                            const float (&correction)[PER], const unsigned char (&group)[PER], float* mine_s, int& chosen) {
+__device__ __forceinline__ bool choose_fast(const GroupRouteArgs& a, const float* zr, float m, double sum, const float (&v)[PER],
+                                            const unsigned char (&group)[PER], float* mine_s, int& chosen) {
   const unsigned all = 0xffffffffu;
   const int lane = threadIdx.x & 31, size = a.size;
-  float v[PER];
-#pragma unroll
-  for (int k = 0; k < PER; ++k) v[k] = score[k] + correction[k];
   unsigned kept = 1;
   if (a.groups > 1) {
     if (a.best > 4) return false;
@@ -276,12 +287,9 @@ __device__ __forceinline__ bool choose_fast(const GroupRouteArgs& a, const float
     unsigned who = __ballot_sync(all, in);
     if (PER > 1 && __any_sync(all, key[PER > 1 ? 1 : 0] >= near)) return false;
     if (who & (who - 1)) {
-      float zi = 0.0f, ci = 0.0f;
-#pragma unroll
-      for (int k = 0; k < PER; ++k)
-        if (k == (int)(key[0] & kLow)) { zi = z[k]; ci = correction[k]; }
-      double most = in ? exact_score(a, zi, m, sum) + (double)ci : -INFINITY;
-      int at = in ? lane + 32 * (int)(key[0] & kLow) : 0x7fffffff;
+      const int i = lane + 32 * (int)(key[0] & kLow);
+      double most = in ? exact_score(a, logit(a, zr, i), m, sum) + (a.correction ? (double)a.correction[i] : 0.0) : -INFINITY;
+      int at = in ? i : 0x7fffffff;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
         const double other = __shfl_xor_sync(all, most, o);
@@ -353,16 +361,16 @@ __global__ void __launch_bounds__(32 * kGroupRouteWarps) moe_route_groups_kernel
       score[k] = z[k] == z[k] ? s : z[k];
     }
   }
+#pragma unroll
+  for (int k = 0; k < PER; ++k) score[k] += correction[k];
   int mine_at = 0;
-  if (!choose_fast<PER>(a, z, m, sum, score, correction, group, reinterpret_cast<float*>(mine_s), mine_at)) {
+  if (!choose_fast<PER>(a, zr, m, sum, score, group, reinterpret_cast<float*>(mine_s), mine_at)) {
     __syncwarp();
-    mine_at = choose_exactly<PER>(a, z, correction, group, mine_s);
+    mine_at = choose_exactly<PER>(a, zr, mine_s);
   }
   double w = 0.0;
   if (lane < a.top) {
-    float zi = zr[mine_at];
-    for (int s = 1; s < a.splits; ++s) zi += zr[s * a.split_stride + mine_at];
-    w = exact_score(a, zi, m, sum);
+    w = exact_score(a, logit(a, zr, mine_at), m, sum);
   }
   if (a.normalized) {
     const double total = warp_sum_f64(w) + (double)a.floor;
