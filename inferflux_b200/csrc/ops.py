@@ -2223,13 +2223,14 @@ class CudaKernels:
             step = softplus(dt + bias);  h[n] <- exp(-step e^log_rate[c, n]) h[n] + step x B[n];  y = (sum_n C[n] h[n] + skip[c] x) silu(z)
         x [T, channels], z (or None: no gate) of its dtype, dt: float32 or bfloat16, rows may be slices of wider rows; bc: float32 [T, 2 states],
         B | C; log_rate: float32 [channels, states]; bias, skip: float32 [channels] or None.  Up to 128 states.  Returns y in
-        `out_dtype` (default x's).  The requests of a step are in slots of their own; a request without tokens keeps its state."""
+        `out_dtype` (default x's); rows behind the last request's are not written.  The requests of a step are in slots of their own; a
+        request without tokens keeps its state."""
         if out_dtype is None:
             out_dtype = x.dtype
         shape, x_code, dt_code, out_code, cu, slots, R = (x.shape, _DT.get(x.dtype), _DT.get(dt.dtype), _DT.get(out_dtype), ctx.cu_seqlens, ctx.req_slot,
                                                           ctx.num_requests)
         # one look at what is usual; what is not is looked at in its turn, for the message
-        f32, i32, C, N = torch.float32, torch.int32, shape[-1], log_rate.shape[-1]
+        f32, i32, C, N = torch.float32, torch.int32, shape[-1] if shape else 0, log_rate.shape[-1] if log_rate.dim() else 0
         ld_x, one_x = x.stride()[-2:] if len(shape) == 2 else (0, 0)
         ld_dt, one_dt = dt.stride() if dt.shape == shape and one_x else (0, 0)
         ld_bc, one_bc = bc.stride()[-2:] if bc.dim() == 2 else (0, 0)

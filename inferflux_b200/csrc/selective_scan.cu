@@ -155,37 +155,34 @@ struct LaneToken {
   }
 };
 
-// Four neighbouring channels of a row as they lie in memory.
+// Four neighbouring channels of a row as they lie in memory: float32, two bfloat16 in each of the first two words, or one by one (SPREAD),
+// a bfloat16 in each word, so that nothing has to wait for a read where rows cannot be read by four.
 struct FourRaw { uint4 v; };
 
-__device__ __forceinline__ FourRaw load_four(const void* p, long long at, int dtype, bool wide, int left) {
+__device__ __forceinline__ FourRaw load_spread(const void* p, int dtype, bool wide, int left) {
   FourRaw r;
   r.v = make_uint4(0u, 0u, 0u, 0u);
   if (dtype == IFX_DT_F32) {
-    const uint32_t* q = static_cast<const uint32_t*>(p) + at;
+    const uint32_t* q = static_cast<const uint32_t*>(p);
     if (wide && left >= 4) return FourRaw{*reinterpret_cast<const uint4*>(q)};
     if (left > 0) r.v.x = q[0];
     if (left > 1) r.v.y = q[1];
     if (left > 2) r.v.z = q[2];
     if (left > 3) r.v.w = q[3];
   } else {
-    const unsigned short* q = static_cast<const unsigned short*>(p) + at;
-    if (wide && left >= 4) {
-      const uint2 two = *reinterpret_cast<const uint2*>(q);
-      r.v.x = two.x;
-      r.v.y = two.y;
-      return r;
-    }
+    const unsigned short* q = static_cast<const unsigned short*>(p);
     if (left > 0) r.v.x = q[0];
-    if (left > 1) r.v.x |= (uint32_t)q[1] << 16;
-    if (left > 2) r.v.y = q[2];
-    if (left > 3) r.v.y |= (uint32_t)q[3] << 16;
+    if (left > 1) r.v.y = q[1];
+    if (left > 2) r.v.z = q[2];
+    if (left > 3) r.v.w = q[3];
   }
   return r;
 }
 
+template <bool SPREAD>
 __device__ __forceinline__ float4 four_f32(const FourRaw& r, int dtype) {
   if (dtype == IFX_DT_F32) return make_float4(__uint_as_float(r.v.x), __uint_as_float(r.v.y), __uint_as_float(r.v.z), __uint_as_float(r.v.w));
+  if (SPREAD) return make_float4(__uint_as_float(r.v.x << 16), __uint_as_float(r.v.y << 16), __uint_as_float(r.v.z << 16), __uint_as_float(r.v.w << 16));
   return make_float4(__uint_as_float(r.v.x << 16), __uint_as_float(r.v.x & 0xffff0000u), __uint_as_float(r.v.y << 16),
                      __uint_as_float(r.v.y & 0xffff0000u));
 }
@@ -474,8 +471,8 @@ __global__ void __launch_bounds__(kSpanThreads, 1) selective_span_kernel(const S
   constexpr int kStride = kWorkers / (CH / 4);                           // tokens from one of a thread's to the next
   static_assert(K == 1 || K * kStride == TT, "a tile's tokens are shared out evenly");
   float4 bias = make_float4(0.0f, 0.0f, 0.0f, 0.0f), skip = bias;
-  if (a.bias) bias = four_f32(load_four(a.bias, c0 + f4, IFX_DT_F32, false, left), IFX_DT_F32);
-  if (a.skip) skip = four_f32(load_four(a.skip, c0 + f4, IFX_DT_F32, false, left), IFX_DT_F32);
+  if (a.bias) bias = four_f32<true>(load_spread(a.bias + c0 + f4, IFX_DT_F32, false, left), IFX_DT_F32);
+  if (a.skip) skip = four_f32<true>(load_spread(a.skip + c0 + f4, IFX_DT_F32, false, left), IFX_DT_F32);
   pdl_wait();
   if (tiles <= 0) return;
   if constexpr (PAD) {
@@ -501,6 +498,8 @@ __global__ void __launch_bounds__(kSpanThreads, 1) selective_span_kernel(const S
   static_assert(PAD || kPieces * kWorkers == TT * NP / 2 || kPieces == 1, "pieces are shared out evenly");
   const int piece_row = tid / (NP / 2), piece_col = tid % (NP / 2) * 4;
   const float* from_bc = a.bc + (first + piece_row) * a.ld_bc + piece_col;
+  FourRaw hold[KNOWN ? 1 : K][3];                                        // rows that cannot be copied by four: a tile's, on their way
+  int held = -1;                                                         // its stage
   auto fetch = [&](int t0, int to) {                                     // one group of copies
     const bool whole = t0 + TT <= n;
     if (!PAD && (a.wide & 8)) {
@@ -522,6 +521,14 @@ __global__ void __launch_bounds__(kSpanThreads, 1) selective_span_kernel(const S
     }
     if (left > 0) {
       char* const stage = stages + to * kStage;
+      if constexpr (!KNOWN) {                                            // what was asked for a tile ago goes to its place
+        if (held >= 0)
+#pragma unroll
+          for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int j = 0; j < 3; ++j) *reinterpret_cast<uint4*>(place(stages + held * kStage, j, k)) = hold[k][j].v;
+        held = to;
+      }
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         if (!whole && t0 + ft + k * kStride >= n) break;
@@ -530,13 +537,9 @@ __global__ void __launch_bounds__(kSpanThreads, 1) selective_span_kernel(const S
           copy_async<XB>(place(stage, 0, k), from_x + k * kStride * row_x, true);
           if (gated) copy_async<XB>(place(stage, 1, k), from_z + k * kStride * row_z, true);
         } else {
-          const FourRaw d = load_four(from_dt + k * kStride * row_dt, 0, dt_dtype, a.wide & 2, left);
-          const FourRaw x = load_four(from_x + k * kStride * row_x, 0, x_dtype, a.wide & 1, left);
-          FourRaw z = x;
-          if (gated) z = load_four(from_z + k * kStride * row_z, 0, x_dtype, a.wide & 4, left);
-          *reinterpret_cast<uint4*>(place(stage, 2, k)) = d.v;
-          *reinterpret_cast<uint4*>(place(stage, 0, k)) = x.v;
-          *reinterpret_cast<uint4*>(place(stage, 1, k)) = z.v;
+          hold[k][2] = load_spread(from_dt + k * kStride * row_dt, dt_dtype, a.wide & 2, left);
+          hold[k][0] = load_spread(from_x + k * kStride * row_x, x_dtype, a.wide & 1, left);
+          if (gated) hold[k][1] = load_spread(from_z + k * kStride * row_z, x_dtype, a.wide & 4, left);
         }
       }
       from_x += TT * row_x;
@@ -551,7 +554,7 @@ __global__ void __launch_bounds__(kSpanThreads, 1) selective_span_kernel(const S
     float4* const to = reinterpret_cast<float4*>(step_s + (buffer * TT + ft) * CH + f4);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const float4 x = four_f32(read_four<XB>(place(stage, 0, k)), x_dtype), raw = four_f32(read_four<DB>(place(stage, 2, k)), dt_dtype);
+      const float4 x = four_f32<!KNOWN>(read_four<XB>(place(stage, 0, k)), x_dtype), raw = four_f32<!KNOWN>(read_four<DB>(place(stage, 2, k)), dt_dtype);
       const float4 step = make_float4(softplus_f32(raw.x + bias.x), softplus_f32(raw.y + bias.y), softplus_f32(raw.z + bias.z), softplus_f32(raw.w + bias.w));
       to[k * kStride * CH / 2] = make_float4(step.x, step.x * x.x, step.y, step.y * x.y);
       to[k * kStride * CH / 2 + 1] = make_float4(step.z, step.z * x.z, step.w, step.w * x.w);
@@ -568,7 +571,7 @@ __global__ void __launch_bounds__(kSpanThreads, 1) selective_span_kernel(const S
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       if (t0 + TT > n && t0 + ft + k * kStride >= n) break;
-      const float4 x = four_f32(read_four<XB>(place(stage, 0, k)), x_dtype);
+      const float4 x = four_f32<!KNOWN>(read_four<XB>(place(stage, 0, k)), x_dtype);
       float out[4];
       lanes_sum<LANES>(sums + k * kStride * CH, PLANE, out);
       if (a.skip) {                                                      // (no skip is not one of zero: x may be infinite)
@@ -578,7 +581,7 @@ __global__ void __launch_bounds__(kSpanThreads, 1) selective_span_kernel(const S
         out[3] = fmaf(skip.w, x.w, out[3]);
       }
       if (gated) {
-        const float4 z = four_f32(read_four<XB>(place(stage, 1, k)), x_dtype);
+        const float4 z = four_f32<!KNOWN>(read_four<XB>(place(stage, 1, k)), x_dtype);
         out[0] *= silu_f32(z.x);
         out[1] *= silu_f32(z.y);
         out[2] *= silu_f32(z.z);

@@ -263,3 +263,54 @@ def test_nothing_to_do(cuda_kernels):
     assert cuda_kernels.selective_scan(d.x, d.dt, d.bc, d.log_rate, d.state, _ctx((0, 0))).shape == (0, 16)
     low, bc = cuda_kernels.selective_inputs(torch.empty(0, 24, device=DEV), 16, 4, F32)
     assert low.shape == (0, 16) and bc.shape == (0, 8) and torch.equal(d.state, before)
+
+
+def test_stretches_on_two_streams_and_in_two_graphs(cuda_kernels):
+    """Long spans of few channels go through scratch of their own in every call, captured or not."""
+    lens = (900, 1, 300)
+    ctx = _ctx(lens, dtype=BF16)
+    data = [_data(sum(lens), 64, 16, 3, BF16, seed=s) for s in (5, 6)]
+    assert cuda_kernels.lib.ifx_selective_scan_scratch(3, 900, 64, 16) > 0
+
+    def scan(d, state):
+        return cuda_kernels.selective_scan(d.x, d.dt, d.bc, d.log_rate, state, ctx, z=d.z, bias=d.bias, skip=d.skip)
+    states = [d.state.clone() for d in data]
+    want = [scan(d, s) for d, s in zip(data, states)]
+    torch.cuda.synchronize()
+    again, got, streams = [d.state.clone() for d in data], [None, None], [torch.cuda.Stream(), torch.cuda.Stream()]
+    for i in range(2):
+        streams[i].wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(streams[i]):
+            got[i] = scan(data[i], again[i])
+    torch.cuda.synchronize()
+    graphs, outs, held = [], [], [d.state.clone() for d in data]
+    for d, s in zip(data, held):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(scan(d, s))
+        graphs.append(g)
+    for d, s in zip(data, held):
+        s.copy_(d.state)
+    torch.cuda.synchronize()
+    for i in range(2):                                      # at the same time
+        with torch.cuda.stream(streams[i]):
+            graphs[i].replay()
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert torch.equal(got[i], want[i]) and torch.equal(again[i], states[i])
+        assert torch.equal(outs[i], want[i]) and torch.equal(held[i], states[i])
+
+
+def test_stretches_meet_the_walk(cuda_kernels):
+    """A span by stretches and the same one walked whole (its scratch left out by the switch): as near as both are to 64 bits."""
+    for lens, C, N in (((1500,), 72, 16), ((257,), 130, 8), ((640, 2, 256, 31), 33, 5), ((1024, 512), 16, 64)):
+        ctx, d = _ctx(lens, dtype=BF16), _data(sum(lens), C, N, len(lens), BF16)
+        assert cuda_kernels.lib.ifx_selective_scan_scratch(len(lens), max(lens), C, N) > 0
+        state = d.state.clone()
+        _check(cuda_kernels, d, ctx, out_dtype=BF16)
+        d.state.copy_(state)
+        cuda_kernels.chunk_scans = False
+        try:
+            _check(cuda_kernels, d, ctx, out_dtype=BF16)
+        finally:
+            cuda_kernels.chunk_scans = True
