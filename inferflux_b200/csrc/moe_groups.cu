@@ -50,7 +50,8 @@ __device__ __forceinline__ float logit(const GroupRouteArgs& a, const float* zr,
   return z;
 }
 
-__device__ __forceinline__ double exact_score(const GroupRouteArgs& a, float z, float m, double sum) {
+// (one copy for all its callers: the rare ones find it in the instruction cache)
+__device__ __noinline__ double exact_score(const GroupRouteArgs& a, float z, float m, double sum) {
   return !a.softmax ? 1.0 / (1.0 + exp(-(double)z)) : sum == 0.0 ? 0.0 : exp((double)z - (double)m) / sum;
 }
 
@@ -183,8 +184,8 @@ __device__ __noinline__ int choose_exactly(const GroupRouteArgs& a, const float*
   return mine_at;
 }
 
-// The same in float32: false, and nothing said, where two groups' strengths are nearer than their errors and one of them goes, where two
-// experts of one lane are, or where a number is none; experts of different lanes that are near are told apart in float64 on the spot.
+// The same in float32, in which experts and groups that are nearer than their errors are told apart in float64 on the spot.  False, and nothing
+// said, where three experts of one lane are that near, more of a group than its strength counts, or where a number is none.
 //
 // A score is off by less than 2^-21: a sigmoid by (0.76 + 0.5 + 2) 2^-23, of which the fast exponential of x, good to 2 + 1.173 |x| steps, makes
 // s (1 - s) (2 + 1.173 |x|) <= 0.76 of them, the sum half a one, and the fast quotient two; a softmax's, by three roundings of what float64 gave.  v is off
@@ -205,7 +206,7 @@ __device__ __forceinline__ bool choose_fast(const GroupRouteArgs& a, const float
     __syncwarp();
     const int g = lane >> a.lane_bits, sub = lane & (a.lanes - 1);
     const float* members = mine_s + min(g, a.groups - 1) * a.stride;
-    float strength, magnitude;                               // of its terms
+    float strength, magnitude, least_term = 0.0f;            // of its terms
     bool numbers = true;                                     // (the largest of a NaN and a number is the number)
     if (a.best <= 2) {
       float first = -INFINITY, next = -INFINITY;
@@ -222,6 +223,7 @@ __device__ __forceinline__ bool choose_fast(const GroupRouteArgs& a, const float
       }
       strength = a.best == 1 ? first : first + next;
       magnitude = fabsf(first) + (a.best == 1 ? 0.0f : fabsf(next));
+      least_term = a.best == 1 ? first : next;
     } else {
       float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
       auto insert = [&](float w) {
@@ -256,7 +258,35 @@ __device__ __forceinline__ bool choose_fast(const GroupRouteArgs& a, const float
       const float inside = from_ordered(__reduce_min_sync(all, in ? ordered_bits(strength) : 0xffffffffu));
       const float outside = from_ordered(__reduce_max_sync(all, lane < a.groups && !in ? ordered_bits(strength) : 0u));
       const float most = __uint_as_float(__reduce_max_sync(all, __float_as_uint(magnitude)));
-      if (__popc(kept) != a.kept || !(inside - outside > (a.best + 1) * 0x1p-20f + most * 0x1p-20f)) return false;
+      const float error = 0x1p-20f + most * 0x1p-20f;        // of two terms; of two strengths so many times as they have terms, and one for their sums
+      if (!(most < INFINITY)) return false;
+      if (__popc(kept) != a.kept || !(inside - outside > (a.best + 1) * error)) {
+        // every group's strength from its largest terms in float64, if those are clear
+        if (a.best > 2) return false;
+        double exact = 0.0;
+        int terms = 0;
+#pragma unroll 1
+        for (int k = 0; k < PER; ++k) {
+          const int i = lane + 32 * k, of = i < a.n ? (int)(i * a.by_size >> 20) : 0;
+          const float line = __shfl_sync(all, least_term, of << a.lane_bits);
+          const bool counts = i < a.n && mine_s[of * a.stride + i - of * size] >= line - error;
+          unsigned who = __ballot_sync(all, counts);
+          if (who == 0) continue;
+          const double term = counts ? exact_score(a, logit(a, zr, i), m, sum) + (a.correction ? (double)a.correction[i] : 0.0) : 0.0;
+          for (; who; who &= who - 1) {
+            const int from = __ffs(who) - 1, to = __shfl_sync(all, of, from);
+            const double more = __shfl_sync(all, term, from);
+            if (lane == to) { exact += more; ++terms; }
+          }
+        }
+        if (!__all_sync(all, lane >= a.groups || terms == a.best)) return false;
+        place = 0;
+        for (int j = 0; j < a.groups; ++j) {
+          const double other = __shfl_sync(all, exact, j);
+          place += other > exact || (other == exact && j < lane);
+        }
+        kept = __ballot_sync(all, lane < a.groups && place < a.kept);
+      }
     }
   }
   // a lane's candidates (0: none) in falling order, each with its number k in the low bits, which the order's last bits give way to
@@ -281,15 +311,31 @@ __device__ __forceinline__ bool choose_fast(const GroupRouteArgs& a, const float
   for (int c = 0; c < a.top; ++c) {
     const float value = from_ordered(__reduce_max_sync(all, key[0]) & ~kLow);
     if (!(value - value == 0.0f)) return false;              // no number
-    // those that may be the largest: alone, or told apart in float64 where they are in lanes of their own
+    // those that may be the largest: one alone, or told apart in float64, of a lane's first two at most
     const unsigned near = ordered_bits(value - (0x1p-20f + fabsf(value) * (0x1p-20f + PER * 0x1p-22f)));
     const bool in = key[0] >= near;                          // (truncated keys on one side only: their last bits are in the bound)
     unsigned who = __ballot_sync(all, in);
-    if (PER > 1 && __any_sync(all, key[PER > 1 ? 1 : 0] >= near)) return false;
-    if (who & (who - 1)) {
-      const int i = lane + 32 * (int)(key[0] & kLow);
-      double most = in ? exact_score(a, logit(a, zr, i), m, sum) + (a.correction ? (double)a.correction[i] : 0.0) : -INFINITY;
-      int at = in ? i : 0x7fffffff;
+    const bool two = PER > 1 && key[PER > 1 ? 1 : 0] >= near;
+    if ((who & (who - 1)) || (PER > 1 && __any_sync(all, two))) {
+      if (PER > 2 && __any_sync(all, key[PER > 2 ? 2 : 0] >= near)) return false;
+      double most = -INFINITY;
+      int at = 0x7fffffff;
+#pragma unroll 1
+      for (int j = 0; j < (PER > 1 ? 2 : 1); ++j) {
+        const int i = lane + 32 * (int)(key[PER > 1 && j ? 1 : 0] & kLow);
+        if (j ? two : in) {
+          const double other = exact_score(a, logit(a, zr, i), m, sum) + (a.correction ? (double)a.correction[i] : 0.0);
+          if (other > most || (other == most && i < at)) {
+            if (j) {                                         // the second is the first
+              const unsigned swap = key[0];
+              key[0] = key[PER > 1 ? 1 : 0];
+              key[PER > 1 ? 1 : 0] = swap;
+            }
+            most = other;
+            at = i;
+          }
+        }
+      }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
         const double other = __shfl_xor_sync(all, most, o);

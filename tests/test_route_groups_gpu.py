@@ -119,3 +119,46 @@ def test_numbers_of_all_sizes(cuda_kernels):
     _same(cuda_kernels, wide, None, top=16, groups=8, kept=4, best=2, score="softmax", floor=1e-20)
     _same(cuda_kernels, wide.clamp(-30, 30), 0.1 * torch.randn(512, generator=g), top=16, groups=8, kept=4, best=2, score="sigmoid")
     _same(cuda_kernels, torch.randn(64, 1024, generator=g), None, top=32, groups=32, kept=32, best=2, score="sigmoid")
+
+
+def _near(k, z, correction, top, groups, kept, best, score):
+    """As in 64 bits, where 64 bits can tell.  Of logits some float32 steps d apart, two pairs' sums differ by as little as s'' d^2 = 0.06 (6e-8)^2 =
+    2e-16, and each side's terms are off by up to a step of 64 bits, 2^-53 for scores below one: two of a strength and one for its sum, on both sides,
+    so strengths within 2^-50 may be taken either way.  Then the choice has to be right for the groups that were taken."""
+    ids, w = k.moe_route_groups(z.to(DEV), None if correction is None else correction.to(DEV), top=top, groups=groups, kept=kept, best=best, score=score)
+    want, _ = PlainKernels().moe_route_groups(z, correction, top=top, groups=groups, kept=kept, best=best, score=score)
+    ids, size = ids.cpu().long(), z.shape[1] // groups
+    s = torch.sigmoid(z.double()) if score == "sigmoid" else torch.softmax(z.double(), 1)
+    v = s if correction is None else s + correction.double()
+    strength = v.view(len(z), groups, size).sort(dim=2, descending=True).values[:, :, :best].sum(2)
+    line = strength.sort(dim=1, descending=True).values[:, kept - 1:kept]
+    slack = 2.0 ** -50
+    for t in (ids != want.long()).any(1).nonzero()[:, 0].tolist():
+        taken = set((ids[t] // size).tolist())
+        assert len(taken) <= kept and all(float(strength[t, g]) >= float(line[t]) - slack for g in taken), t
+        # groups without a chosen expert may be among the kept ones too: those that must be, and of the near ones none that need be
+        allowed = taken | {g for g in range(groups) if float(strength[t, g]) > float(line[t]) + slack}
+        assert len(allowed) <= kept, t
+        order = [i for i in v[t].sort(descending=True, stable=True).indices.tolist() if i // size in allowed]
+        assert ids[t].tolist() == order[:top], t
+    return ids, w
+
+
+@pytest.mark.parametrize("n,groups,kept,best,top", [(256, 8, 4, 2, 8), (64, 8, 3, 2, 8), (32, 4, 2, 1, 5), (512, 16, 5, 2, 12), (30, 1, 1, 1, 9), (160, 8, 3, 1, 6)])
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("spread", [1e-7, 1e-6, 1e-5])
+def test_groups_and_experts_all_near(cuda_kernels, n, groups, kept, best, top, score, spread):
+    """Scores within some float32 steps of one another, in one lane's experts, in other lanes', and in whole groups; half of the experts a little
+    further off; corrections that move them by as little."""
+    g = torch.Generator().manual_seed(n + top)
+    z = 0.5 + spread * torch.randn(500, n, generator=g)
+    z[:, ::2] -= 0.01
+    _near(cuda_kernels, z, None, top=top, groups=groups, kept=kept, best=best, score=score)
+    _near(cuda_kernels, z, spread * torch.randn(n, generator=g), top=top, groups=groups, kept=kept, best=best, score=score)
+    rows = 2 * torch.randn(500, n, generator=g)                # rows as they are, but two groups alike but for a step, and two experts
+    size = n // groups
+    if groups > 1:
+        rows[:, size:2 * size] = torch.nextafter(rows[:, :size].flip(1), torch.tensor(9.0))
+    rows[:, n - 1] = torch.nextafter(rows[:, 0], torch.tensor(-9.0))
+    rows[:, n // 2] = rows[:, 1]
+    _near(cuda_kernels, rows, None, top=top, groups=groups, kept=kept, best=best, score=score)
