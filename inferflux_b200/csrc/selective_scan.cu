@@ -608,8 +608,10 @@ __global__ void __launch_bounds__(kSpanThreads, 1) selective_span_kernel(const S
 }
 
 // One token a request at most: a thread has four states of a channel of Q requests, whose rates it makes once; all its reads are under way
-// before the first is looked at (dtypes that a branch chooses are turned into float32 behind the last of them).  WIDE: states, rates, B
-// and C four at a time.  Bound by the states' way in and out: 64 requests of 7,168 channels of 16 states, 62 MB, 15 us, 4.1 TB/s.
+// before the first is looked at (dtypes that a branch chooses are turned into float32 behind the last of them).  What there is once a
+// channel (the step, the gate, the skip, the result's way out) is done by one lane for each request, not by all of them (us: 15.0 for
+// 15.7; 24 requests 5.3 for 5.9).  WIDE: states, rates, B and C four at a time.  Bound by the states' way in and out: 64 requests of
+// 7,168 channels of 16 states, 62 MB, 15.0 us, 4.2 TB/s.
 template <int LANES, bool PAD, bool WIDE, int Q>
 __global__ void __launch_bounds__(kStepThreads) selective_step_kernel(const SelectiveArgs a, int requests) {
   constexpr int S = kLaneStates, CH = kStepThreads / LANES;
@@ -617,54 +619,63 @@ __global__ void __launch_bounds__(kStepThreads) selective_step_kernel(const Sele
   const int c = min(c_mine, a.channels - 1);                 // (threads behind the last channel read it, and store nothing)
   pdl_launch_dependents();
   LaneStates<S> rate2, h[Q], b[Q], c_[Q];
-  uint32_t x_raw[Q], dt_raw[Q], z_raw[Q];
   auto get = [&](LaneStates<S>& to, const float* from) {
     if (WIDE) to.load_wide(from);
     else to.load(from, real);
   };
   get(rate2, a.log_rate + (long long)c * a.states + part * S);
   const float bias = a.bias ? a.bias[c] : 0.0f, skip = a.skip ? a.skip[c] : 0.0f;
-  int t[Q], behind[Q], slot[Q];
+  // what there is once a channel is done for request `own` alone, and handed to the channel's other lanes
+  const int own = part % Q;
+  int t[Q], t_own = 0;
+  bool any[Q], any_own = false;
+  float* st[Q];
 #pragma unroll
   for (int q = 0; q < Q; ++q) {
     const int r = min(r0 + q, requests - 1);
     t[q] = a.cu_seqlens[r];
-    behind[q] = r0 + q < requests ? a.cu_seqlens[r + 1] : t[q];
-    slot[q] = a.req_slot[r];
+    any[q] = r0 + q < requests && a.cu_seqlens[r + 1] > t[q];
+    st[q] = a.state + (long long)a.req_slot[r] * a.slot_stride + (long long)c * a.states + part * S;
+    if (q == own) { t_own = t[q]; any_own = any[q]; }
   }
   pdl_wait();
+  uint32_t x_raw = 0u, dt_raw = 0u, z_raw = 0u;
+  if (any_own) {
+    x_raw = load_raw(a.x, t_own * a.ld_x + c, a.x_dtype);
+    dt_raw = load_raw(a.dt, t_own * a.ld_dt + c, a.dt_dtype);
+    if (a.z) z_raw = load_raw(a.z, t_own * a.ld_z + c, a.x_dtype);
+  }
 #pragma unroll
   for (int q = 0; q < Q; ++q) {
-    if (behind[q] <= t[q]) continue;
-    get(h[q], a.state + (long long)slot[q] * a.slot_stride + (long long)c * a.states + part * S);
-    x_raw[q] = load_raw(a.x, t[q] * a.ld_x + c, a.x_dtype);
-    dt_raw[q] = load_raw(a.dt, t[q] * a.ld_dt + c, a.dt_dtype);
-    z_raw[q] = a.z ? load_raw(a.z, t[q] * a.ld_z + c, a.x_dtype) : 0u;
+    if (!any[q]) continue;                                               // (the same for a whole block)
+    get(h[q], st[q]);
     get(b[q], a.bc + t[q] * a.ld_bc + part * S);
     get(c_[q], a.bc + t[q] * a.ld_bc + a.states + part * S);
   }
   rate2.to_rate2();
+  const float x = raw_f32(x_raw, a.x_dtype), step = softplus_f32(raw_f32(dt_raw, a.dt_dtype) + bias), in = step * x;
+  float y_own = 0.0f;
 #pragma unroll
   for (int q = 0; q < Q; ++q) {
-    if (behind[q] <= t[q]) continue;
-    const float x = raw_f32(x_raw[q], a.x_dtype), step = softplus_f32(raw_f32(dt_raw[q], a.dt_dtype) + bias);
+    if (!any[q]) continue;
+    const float step_q = Q == 1 ? step : __shfl_sync(0xffffffffu, step, q, LANES), in_q = Q == 1 ? in : __shfl_sync(0xffffffffu, in, q, LANES);
     LaneToken<S> token;
-    token.make(rate2, step, step * x, b[q]);
+    token.make(rate2, step_q, in_q, b[q]);
     float y = token.template go<PAD>(h[q], c_[q], real);
 #pragma unroll
     for (int o = 1; o < LANES; o <<= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
-    if (c_mine >= a.channels) continue;
-    float* st = a.state + (long long)slot[q] * a.slot_stride + (long long)c * a.states + part * S;
-    if (WIDE) h[q].store_wide(st);
-    else h[q].store(st, real);
-    if (part == 0) {
-      if (a.skip) y = fmaf(skip, x, y);
-      if (a.z) y *= silu_f32(raw_f32(z_raw[q], a.x_dtype));
-      const long long at = (long long)t[q] * a.channels + c;
-      if (a.out_dtype == IFX_DT_F32) static_cast<float*>(a.out)[at] = y;
-      else static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(y);
+    if (q == own) y_own = y;
+    if (c_mine < a.channels) {
+      if (WIDE) h[q].store_wide(st[q]);
+      else h[q].store(st[q], real);
     }
   }
+  if (part >= Q || !any_own || c_mine >= a.channels) return;
+  if (a.skip) y_own = fmaf(skip, x, y_own);
+  if (a.z) y_own *= silu_f32(raw_f32(z_raw, a.x_dtype));
+  const long long at = (long long)t_own * a.channels + c;
+  if (a.out_dtype == IFX_DT_F32) static_cast<float*>(a.out)[at] = y_own;
+  else static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(y_own);
 }
 
 struct SelectiveInputsArgs {
@@ -796,10 +807,11 @@ static int launch_selective(SelectiveArgs a, int requests, int max_span, int str
     const long long blocks = (a.channels + kChannels - 1) / kChannels;
     const bool wide = !PAD && (a.wide & 104) == 104;
     // two requests a thread share its rates; with few requests one, for the shorter way (us, 7,168 channels: 1 request 1.6 / 1.8, 8 3.2 / 3.3, 24
-    // 7.1 / 5.9, 64 18 / 15)
-    const int each = requests >= 12 ? 2 : 1;
-    auto kernel = each == 2 ? (wide ? selective_step_kernel<LANES, PAD, !PAD, 2> : selective_step_kernel<LANES, PAD, false, 2>)
-                            : (wide ? selective_step_kernel<LANES, PAD, !PAD, 1> : selective_step_kernel<LANES, PAD, false, 1>);
+    // 7.1 / 5.3, 64 18 / 15)
+    constexpr int kMost = LANES >= 2 ? 2 : 1;
+    const int each = requests >= 12 ? kMost : 1;
+    auto kernel = each == kMost ? (wide ? selective_step_kernel<LANES, PAD, !PAD, kMost> : selective_step_kernel<LANES, PAD, false, kMost>)
+                                : (wide ? selective_step_kernel<LANES, PAD, !PAD, 1> : selective_step_kernel<LANES, PAD, false, 1>);
     return launch_pdl(kernel, dim3((unsigned)blocks, (unsigned)((requests + each - 1) / each)), dim3(kStepThreads), 0, stream, 1, a, requests);
   }
   using Tile = SpanTile<LANES>;
