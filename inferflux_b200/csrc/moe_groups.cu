@@ -22,7 +22,7 @@ struct GroupRouteArgs {
   float floor, scale;
 };
 
-constexpr int kGroupRouteMost = 1024, kGroupRouteWarps = 4;
+constexpr int kGroupRouteMost = 1024, kGroupRouteWarps = 2;
 
 // Bits ordered as the numbers are, of numbers alone (one zero); 0 stands before all of them.
 __device__ __forceinline__ unsigned long long ordered_bits(double v) {
@@ -55,10 +55,9 @@ __device__ __noinline__ double exact_score(const GroupRouteArgs& a, float z, flo
   return !a.softmax ? 1.0 / (1.0 + exp(-(double)z)) : sum == 0.0 ? 0.0 : exp((double)z - (double)m) / sum;
 }
 
-// One token by a warp, whose lane has the experts lane, lane + 32, ... (PER of them at most).  zr: its logits.  Both give the choice, number c
-// in lane c.
+// One token by a warp.  zr: its logits.  Both give the choice, number c in lane c.
 //
-// In float64: every v goes to shared memory, group by group; a group's lanes find its two largest (more: its first lane does, one after the
+// In float64, where a lane has the experts lane, lane + 32, ... (PER of them at most): every v goes to shared memory, group by group; a group's lanes find its two largest (more: its first lane does, one after the
 // other), and the choice goes through registers: the largest high words by one reduction, the low words and then the indices where those are
 // equal.
 template <int PER>
@@ -184,37 +183,43 @@ __device__ __noinline__ int choose_exactly(const GroupRouteArgs& a, const float*
   return mine_at;
 }
 
+// Where a lane's experts are in choose_fast: `lanes` lanes have a group, so that its strength takes registers alone.
+struct GroupLane {
+  int first, count, bits;                                    // its k-th of `count` is expert first + (k << bits)
+  __device__ __forceinline__ explicit GroupLane(const GroupRouteArgs& a) : bits(a.lane_bits) {
+    const int lane = threadIdx.x & 31, g = lane >> a.lane_bits, sub = lane & (a.lanes - 1);
+    first = g * a.size + sub;
+    count = g < a.groups ? (a.size - sub + a.lanes - 1) >> a.lane_bits : 0;
+  }
+  __device__ __forceinline__ int at(int k) const { return first + (k << bits); }
+};
+
 // The same in float32, in which experts and groups that are nearer than their errors are told apart in float64 on the spot.  False, and nothing
 // said, where three experts of one lane are that near, more of a group than its strength counts, or where a number is none.
+// v: -inf behind the lane's last.
 //
 // A score is off by less than 2^-21: a sigmoid by (0.76 + 0.5 + 2) 2^-23, of which the fast exponential of x, good to 2 + 1.173 |x| steps, makes
 // s (1 - s) (2 + 1.173 |x|) <= 0.76 of them, the sum half a one, and the fast quotient two; a softmax's, by three roundings of what float64 gave.  v is off
 // by half a step of its own more, a strength by its terms' errors and a rounding a sum.
 template <int PER>
 __device__ __forceinline__ bool choose_fast(const GroupRouteArgs& a, const float* zr, float m, double sum, const float (&v)[PER],
-                                            const unsigned char (&group)[PER], float* mine_s, int& chosen) {
+                                            const GroupLane& own, int& chosen) {
   const unsigned all = 0xffffffffu;
-  const int lane = threadIdx.x & 31, size = a.size;
-  unsigned kept = 1;
+  const int lane = threadIdx.x & 31;
+  bool in_kept = true;
   if (a.groups > 1) {
     if (a.best > 4) return false;
-#pragma unroll
-    for (int k = 0; k < PER; ++k) {
-      const int i = lane + 32 * k;
-      if (i < a.n) mine_s[group[k] * a.stride + i - group[k] * size] = v[k];
-    }
-    __syncwarp();
-    const int g = lane >> a.lane_bits, sub = lane & (a.lanes - 1);
-    const float* members = mine_s + min(g, a.groups - 1) * a.stride;
     float strength, magnitude, least_term = 0.0f;            // of its terms
     bool numbers = true;                                     // (the largest of a NaN and a number is the number)
+#pragma unroll
+    for (int k = 0; k < PER; ++k) numbers = numbers && v[k] == v[k];
+    if (!__all_sync(all, numbers)) return false;
     if (a.best <= 2) {
       float first = -INFINITY, next = -INFINITY;
-      for (int i = sub; i < size; i += a.lanes) {
-        const float w = members[i];
-        numbers = numbers && w == w;
-        next = fmaxf(next, fminf(first, w));
-        first = fmaxf(first, w);
+#pragma unroll
+      for (int k = 0; k < PER; ++k) {
+        next = fmaxf(next, fminf(first, v[k]));
+        first = fmaxf(first, v[k]);
       }
       for (int o = 1; o < a.lanes; o <<= 1) {
         const float other = __shfl_xor_sync(all, first, o);
@@ -234,10 +239,8 @@ __device__ __forceinline__ bool choose_fast(const GroupRouteArgs& a, const float
           w = less;
         }
       };
-      for (int i = sub; i < size; i += a.lanes) {
-        numbers = numbers && members[i] == members[i];
-        insert(members[i]);
-      }
+#pragma unroll
+      for (int k = 0; k < PER; ++k) insert(v[k]);
       for (int o = 1; o < a.lanes; o <<= 1) {
         float other[4];
 #pragma unroll
@@ -248,53 +251,54 @@ __device__ __forceinline__ bool choose_fast(const GroupRouteArgs& a, const float
       strength = top[0] + top[1] + top[2] + (a.best == 4 ? top[3] : 0.0f);
       magnitude = fabsf(top[0]) + fabsf(top[1]) + fabsf(top[2]) + (a.best == 4 ? fabsf(top[3]) : 0.0f);
     }
-    if (!__all_sync(all, numbers)) return false;
-    strength = __shfl_sync(all, strength, min(lane, a.groups - 1) * a.lanes);
+    const bool real = lane >> a.lane_bits < a.groups;        // (lanes behind the last group have none)
     int place = 0;
-    for (int j = 0; j < a.groups; ++j) place += __shfl_sync(all, strength, j) > strength;
-    kept = __ballot_sync(all, lane < a.groups && place < a.kept);
+    for (int j = 0; j < a.groups; ++j) place += __shfl_sync(all, strength, j << a.lane_bits) > strength;
+    in_kept = real && place < a.kept;
     if (a.kept < a.groups) {
-      const bool in = kept >> lane & 1u;
-      const float inside = from_ordered(__reduce_min_sync(all, in ? ordered_bits(strength) : 0xffffffffu));
-      const float outside = from_ordered(__reduce_max_sync(all, lane < a.groups && !in ? ordered_bits(strength) : 0u));
-      const float most = __uint_as_float(__reduce_max_sync(all, __float_as_uint(magnitude)));
+      const int kept = __popc(__ballot_sync(all, in_kept));
+      const float inside = from_ordered(__reduce_min_sync(all, in_kept ? ordered_bits(strength) : 0xffffffffu));
+      const float outside = from_ordered(__reduce_max_sync(all, real && !in_kept ? ordered_bits(strength) : 0u));
+      const float most = __uint_as_float(__reduce_max_sync(all, real ? __float_as_uint(magnitude) : 0u));
       const float error = 0x1p-20f + most * 0x1p-20f;        // of two terms; of two strengths so many times as they have terms, and one for their sums
       if (!(most < INFINITY)) return false;
-      if (__popc(kept) != a.kept || !(inside - outside > (a.best + 1) * error)) {
+      if (kept != a.kept << a.lane_bits || !(inside - outside > (a.best + 1) * error)) {
         // every group's strength from its largest terms in float64, if those are clear
         if (a.best > 2) return false;
+        unsigned long long counts = 0;
+#pragma unroll
+        for (int k = 0; k < PER; ++k)
+          if (k < own.count && v[k] >= least_term - error) counts |= 1ull << k;
         double exact = 0.0;
-        int terms = 0;
-#pragma unroll 1
-        for (int k = 0; k < PER; ++k) {
-          const int i = lane + 32 * k, of = i < a.n ? (int)(i * a.by_size >> 20) : 0;
-          const float line = __shfl_sync(all, least_term, of << a.lane_bits);
-          const bool counts = i < a.n && mine_s[of * a.stride + i - of * size] >= line - error;
-          unsigned who = __ballot_sync(all, counts);
-          if (who == 0) continue;
-          const double term = counts ? exact_score(a, logit(a, zr, i), m, sum) + (a.correction ? (double)a.correction[i] : 0.0) : 0.0;
-          for (; who; who &= who - 1) {
-            const int from = __ffs(who) - 1, to = __shfl_sync(all, of, from);
-            const double more = __shfl_sync(all, term, from);
-            if (lane == to) { exact += more; ++terms; }
+        int terms = __popcll(counts);
+        while (__any_sync(all, counts != 0)) {
+          if (counts) {
+            const int i = own.at(__ffsll(counts) - 1);
+            exact += exact_score(a, logit(a, zr, i), m, sum) + (a.correction ? (double)a.correction[i] : 0.0);
+            counts &= counts - 1;
           }
+          __syncwarp();
         }
-        if (!__all_sync(all, lane >= a.groups || terms == a.best)) return false;
+        for (int o = 1; o < a.lanes; o <<= 1) {              // (two terms' sum: in either order)
+          exact += __shfl_xor_sync(all, exact, o);
+          terms += __shfl_xor_sync(all, terms, o);
+        }
+        if (!__all_sync(all, !real || terms == a.best)) return false;
         place = 0;
         for (int j = 0; j < a.groups; ++j) {
-          const double other = __shfl_sync(all, exact, j);
-          place += other > exact || (other == exact && j < lane);
+          const double other = __shfl_sync(all, exact, j << a.lane_bits);
+          place += other > exact || (other == exact && j < lane >> a.lane_bits);
         }
-        kept = __ballot_sync(all, lane < a.groups && place < a.kept);
+        in_kept = real && place < a.kept;
       }
     }
   }
   // a lane's candidates (0: none) in falling order, each with its number k in the low bits, which the order's last bits give way to
   constexpr unsigned kLow = PER - 1;
   unsigned key[PER];
+  const int candidates = in_kept ? own.count : 0;
 #pragma unroll
-  for (int k = 0; k < PER; ++k)
-    key[k] = lane + 32 * k < a.n && (kept >> group[k] & 1u) ? (ordered_bits(v[k]) & ~kLow) | (unsigned)k : 0u;
+  for (int k = 0; k < PER; ++k) key[k] = k < candidates ? (ordered_bits(v[k]) & ~kLow) | (unsigned)k : 0u;
 #pragma unroll
   for (int length = 2; length <= PER; length *= 2)           // bitonic merges
 #pragma unroll
@@ -322,7 +326,7 @@ __device__ __forceinline__ bool choose_fast(const GroupRouteArgs& a, const float
       int at = 0x7fffffff;
 #pragma unroll 1
       for (int j = 0; j < (PER > 1 ? 2 : 1); ++j) {
-        const int i = lane + 32 * (int)(key[PER > 1 && j ? 1 : 0] & kLow);
+        const int i = own.at((int)(key[PER > 1 && j ? 1 : 0] & kLow));
         if (j ? two : in) {
           const double other = exact_score(a, logit(a, zr, i), m, sum) + (a.correction ? (double)a.correction[i] : 0.0);
           if (other > most || (other == most && i < at)) {
@@ -336,15 +340,16 @@ __device__ __forceinline__ bool choose_fast(const GroupRouteArgs& a, const float
           }
         }
       }
+      const int mine = at;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
         const double other = __shfl_xor_sync(all, most, o);
         const int other_at = __shfl_xor_sync(all, at, o);
         if (other > most || (other == most && other_at < at)) { most = other; at = other_at; }
       }
-      who = 1u << (at & 31);
+      who = __ballot_sync(all, in && mine == at);
     }
-    const int winner = __ffs(who) - 1, at = winner + 32 * (int)(__shfl_sync(all, key[0], winner) & kLow);
+    const int winner = __ffs(who) - 1, at = __shfl_sync(all, own.at((int)(key[0] & kLow)), winner);
     if (lane == c) chosen = at;
     if (lane == winner) {
 #pragma unroll
@@ -355,32 +360,30 @@ __device__ __forceinline__ bool choose_fast(const GroupRouteArgs& a, const float
   return true;
 }
 
-// A warp a token.  Bound by the latency of one token's chain (a decode batch) and by the instructions of all (prompts).
+// A warp a token.  Bound by the latency of one token's chain (a decode batch) and by the instructions of all (prompts).  A lane's experts are
+// all of one group, so that strengths take registers and `lanes` - 1 shuffles, not a row in shared memory (us, 8,192 tokens of 256 experts in 8
+// groups 15.1 for 16.6, 2,047 of 160 5.9 / 6.8, 24 of 256 3.7 / 4.0).  Two warps a block, four, eight: 14.8, 15.1, 15.9; 24 tokens 3.5, 3.7, 4.1.
+// Without the choice's rounds but the first 11.4, without the groups 13.6, with weights in float32 13.7.
 template <int PER>
 __global__ void __launch_bounds__(32 * kGroupRouteWarps) moe_route_groups_kernel(const GroupRouteArgs a) {
   extern __shared__ double v_s[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long t = (long long)blockIdx.x * kGroupRouteWarps + warp;
   pdl_launch_dependents();
+  const GroupLane own(a);
   float correction[PER];
-  unsigned char group[PER];
 #pragma unroll
-  for (int k = 0; k < PER; ++k) {
-    correction[k] = a.correction && lane + 32 * k < a.n ? a.correction[lane + 32 * k] : 0.0f;
-  }
-#pragma unroll
-  for (int k = 0; k < PER; ++k) group[k] = (unsigned char)((lane + 32 * k) * a.by_size >> 20);
+  for (int k = 0; k < PER; ++k) correction[k] = a.correction && k < own.count ? a.correction[own.at(k)] : 0.0f;
   pdl_wait();
   if (t >= a.T) return;
-  double* const mine_s = v_s + (size_t)warp * a.groups * a.stride;
   const float* zr = a.z + t * a.n;
   float z[PER];
 #pragma unroll
-  for (int k = 0; k < PER; ++k) z[k] = lane + 32 * k < a.n ? zr[lane + 32 * k] : -INFINITY;
+  for (int k = 0; k < PER; ++k) z[k] = k < own.count ? zr[own.at(k)] : -INFINITY;
   for (int s = 1; s < a.splits; ++s)
 #pragma unroll
     for (int k = 0; k < PER; ++k)
-      if (lane + 32 * k < a.n) z[k] += zr[s * a.split_stride + lane + 32 * k];
+      if (k < own.count) z[k] += zr[s * a.split_stride + own.at(k)];
   float score[PER], m = 0.0f;
   double sum = 1.0;                                          // (in float64: every weight is rounded once)
   if (a.softmax) {
@@ -408,11 +411,11 @@ __global__ void __launch_bounds__(32 * kGroupRouteWarps) moe_route_groups_kernel
     }
   }
 #pragma unroll
-  for (int k = 0; k < PER; ++k) score[k] += correction[k];
+  for (int k = 0; k < PER; ++k) score[k] = k < own.count ? score[k] + correction[k] : -INFINITY;
   int mine_at = 0;
-  if (!choose_fast<PER>(a, zr, m, sum, score, group, reinterpret_cast<float*>(mine_s), mine_at)) {
+  if (!choose_fast<PER>(a, zr, m, sum, score, own, mine_at)) {
     __syncwarp();
-    mine_at = choose_exactly<PER>(a, zr, mine_s);
+    mine_at = choose_exactly<PER < 32 ? PER : 32>(a, zr, v_s + (size_t)warp * a.groups * a.stride);      // (32 PER >= n)
   }
   double w = 0.0;
   if (lane < a.top) {
@@ -449,9 +452,11 @@ extern "C" int ifx_moe_route_groups(const float* z, int splits, const float* cor
     ++a.lane_bits;
   }
   while (a.stride % 16 != a.lanes % 16) ++a.stride;           // a half warp's reads of 8 bytes fall on different banks
-  const size_t bytes = (size_t)kGroupRouteWarps * groups * a.stride * sizeof(double);       // 32 groups of 32 experts and one: 34 KB; at most 48
+  const size_t bytes = (size_t)kGroupRouteWarps * groups * a.stride * sizeof(double);       // 32 groups of 32 experts and one: 17 KB; at most 24
   const dim3 grid((unsigned)((T + kGroupRouteWarps - 1) / kGroupRouteWarps)), block(32 * kGroupRouteWarps);
-  auto kernel = n <= 32 ? moe_route_groups_kernel<1> : n <= 64 ? moe_route_groups_kernel<2> : n <= 128 ? moe_route_groups_kernel<4>
-              : n <= 256 ? moe_route_groups_kernel<8> : n <= 512 ? moe_route_groups_kernel<16> : moe_route_groups_kernel<32>;
+  const int per = (size + a.lanes - 1) / a.lanes;             // of a lane: up to 60, as 17 groups of 60 have a lane each
+  auto kernel = per <= 1 ? moe_route_groups_kernel<1> : per <= 2 ? moe_route_groups_kernel<2> : per <= 4 ? moe_route_groups_kernel<4>
+              : per <= 8 ? moe_route_groups_kernel<8> : per <= 16 ? moe_route_groups_kernel<16> : per <= 32 ? moe_route_groups_kernel<32>
+                                                                                                          : moe_route_groups_kernel<64>;
   return launch_pdl(kernel, grid, block, groups > 1 ? bytes : 0, stream, 1, a);
 }

@@ -162,3 +162,18 @@ def test_groups_and_experts_all_near(cuda_kernels, n, groups, kept, best, top, s
     rows[:, n - 1] = torch.nextafter(rows[:, 0], torch.tensor(-9.0))
     rows[:, n // 2] = rows[:, 1]
     _near(cuda_kernels, rows, None, top=top, groups=groups, kept=kept, best=best, score=score)
+
+
+@pytest.mark.parametrize("n,groups,kept,best,top", [(8, 8, 3, 1, 3), (24, 8, 5, 2, 9), (12, 4, 2, 3, 6), (950, 19, 4, 2, 12), (1020, 17, 3, 4, 20), (1008, 24, 7, 1, 32),
+                                                    (45, 5, 2, 2, 8), (930, 31, 6, 2, 8), (992, 31, 6, 2, 8), (1024, 1, 1, 1, 32), (1022, 2, 1, 2, 5)])
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+def test_groups_of_every_size(cuda_kernels, n, groups, kept, best, top, score):
+    """Fewer experts in a group than lanes, lanes with none, and up to sixty of a lane; rows as they are, near ones, and some that are no numbers."""
+    g = torch.Generator().manual_seed(n + groups)
+    z, c = 2 * torch.randn(90, n, generator=g), 0.1 * torch.randn(n, generator=g)
+    z[3, 0], z[4], z[5, n - 1], z[6, : n // 2] = math.nan, -math.inf, -math.inf, -math.inf
+    _same(cuda_kernels, z, c, top=top, groups=groups, kept=kept, best=best, score=score)
+    best = min(best, 2)                                      # (what `_near` allows for is of two terms)
+    near = 0.5 + 1e-6 * torch.randn(90, n, generator=g)
+    _near(cuda_kernels, near, None, top=top, groups=groups, kept=kept, best=best, score=score)
+    _near(cuda_kernels, near, 1e-6 * torch.randn(n, generator=g), top=top, groups=groups, kept=kept, best=best, score=score)
