@@ -12,6 +12,7 @@
 // A channel's states are spread over lanes, four a lane.  A lane adds its terms as (0 and 2) and (1 and 3), the lanes' sums are added as a tree,
 // neighbours first, and every h is one chain of multiply-adds from token to token, whichever kernel walks; so a float32 run's bits do not depend
 // on how a request's tokens are cut into steps.
+#include <cfloat>
 #include <type_traits>
 
 #include "common.cuh"
@@ -119,10 +120,15 @@ struct LaneStates {
     if constexpr (S == 4) *reinterpret_cast<float4*>(p) = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
     else *reinterpret_cast<float2*>(p) = v[0];
   }
-  // log_rate in, -e^log_rate log2 e out
+  // log_rate in, -e^log_rate log2 e out, float32's lowest number where that is beyond it: any step of 2^-119 and more makes a decay of 0 of it, and a
+  // step of 0 one of 1, not 0 * -inf.  (A rate that is no number stays none.)
+  __device__ __forceinline__ static float rate2_of(float log_rate) {
+    const float r = -expf(log_rate) * kLog2e;
+    return r < -FLT_MAX ? -FLT_MAX : r;
+  }
   __device__ __forceinline__ void to_rate2() {
 #pragma unroll
-    for (int j = 0; j < S / 2; ++j) v[j] = make_float2(-expf(v[j].x) * kLog2e, -expf(v[j].y) * kLog2e);
+    for (int j = 0; j < S / 2; ++j) v[j] = make_float2(rate2_of(v[j].x), rate2_of(v[j].y));
   }
 };
 
