@@ -2211,9 +2211,10 @@ class CudaKernels:
         low = torch.empty(T, rank, dtype=out_dtype, device=device)
         bc = torch.empty(T, 2 * states, dtype=torch.float32, device=device)
         if T:
-            # (a single row's stride may be anything)
-            _check(self.lib.ifx_selective_inputs(src, max(strides[-2], width), code, splits, w_low, w_b, w_c, eps, low, low_code, bc, T, rank,
-                                                 states, _stream()), "selective_inputs")
+            # (a single row's stride may be anything, and slices lie T times what is said here apart)
+            ld = width if splits > 1 else max(strides[-2], width)
+            _check(self.lib.ifx_selective_inputs(src, ld, code, splits, w_low, w_b, w_c, eps, low, low_code, bc, T, rank, states, _stream()),
+                   "selective_inputs")
             self.launches += 1
         return low, bc
 
