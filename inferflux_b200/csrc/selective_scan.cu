@@ -888,7 +888,7 @@ extern "C" int ifx_selective_scan(const void* x, long long ld_x, int x_dtype, co
   const int lanes = lanes_of(states);
   a.per_block = kWalkers / lanes;
   const int stretches = scratch_floats > 0 ? stretches_of(channels, states, num_requests, max_span) : 0;
-  if (stretches && scratch_floats < stretches * (long long)num_requests * channels * (states + 1)) return IFX_E_BADARG;
+  if (stretches && (!scratch || scratch_floats < stretches * (long long)num_requests * channels * (states + 1))) return IFX_E_BADARG;
   const bool pad = states != lanes * kLaneStates;
 #define IFX_SELECTIVE(L)                                                                        \
   return pad ? launch_selective<L, true>(a, num_requests, max_span, stretches, stream)          \

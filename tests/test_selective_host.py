@@ -1,8 +1,11 @@
 """What the selective scan's and its inputs' entry points hand to the kernels, without a GPU: nothing is launched."""
+import ctypes
+
 import pytest
 import torch
 
 from inferflux_b200.csrc import CudaKernels, ops
+from inferflux_b200.csrc.build import load_library
 from inferflux_b200.csrc.ops import PartialSum
 
 F32 = torch.float32
@@ -44,3 +47,19 @@ def test_slices_of_a_single_row(kernels, splits, T):
     assert name == "ifx_selective_inputs" and args[0] is parts and args[3] == splits
     assert T * args[1] == width * T          # what the kernel takes for the distance between slices
     assert low.shape == (T, rank) and bc.shape == (T, 2 * states)
+
+
+def test_stretches_without_their_scratch():
+    """The C entry point: room that is said to be there, and no address for it, is refused before anything is launched."""
+    lib, p, n = load_library(), ctypes.c_void_p(16), ctypes.c_void_p(0)
+    ll = ctypes.c_longlong
+    T, C, N = 300, 64, 16
+    lib.ifx_selective_scan_scratch.restype = ctypes.c_longlong
+    room = lib.ifx_selective_scan_scratch(1, T, C, N)
+    assert room > 0
+
+    def scan(scratch, floats):
+        return lib.ifx_selective_scan(p, ll(C), 0, p, ll(C), 0, p, ll(2 * N), n, ll(0), p, n, n, p, ll(C * N), p, p, p, 0, 1, T, T, C, N, scratch,
+                                      ll(floats), n)
+    assert scan(n, room) == -1
+    assert scan(p, room - 1) == -1
