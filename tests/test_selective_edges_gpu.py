@@ -92,3 +92,42 @@ def test_a_rate_that_is_no_number(cuda_kernels, lens, dtype):
     bad = d.state.view(40, 16).isnan()
     assert bool(bad[7, 3]) and int(bad.sum()) == 1
     assert torch.equal(d.state.view(40, 16)[~bad], want_state.view(40, 16)[~bad])
+
+
+def _few(k, v, z=None, dtype=F32):
+    """The steps of v [T, C] (times their gates) as the scan gives them: a state of one number from 0, with x, B and C of 1, is the step, in the
+    single-token kernel and in the other one (which a longest span of two tokens stands for)."""
+    T, C = v.shape
+    one, bc, rate = torch.ones(T, C, device=DEV, dtype=dtype), torch.ones(T, 2, device=DEV), torch.full((C, 1), math.inf, device=DEV)
+    ctx, got = _ctx((1,) * T), []
+    for ctx.max_span in (1, 2):
+        got.append(k.selective_scan(one, v, bc, rate, torch.zeros(T, C, device=DEV), ctx, z=z, out_dtype=F32))
+    assert torch.equal(got[0].isnan(), got[1].isnan()) and torch.equal(got[0].nan_to_num(), got[1].nan_to_num())
+    return got[0]
+
+
+@pytest.mark.parametrize("lo,hi", [(-85, -20), (-20, -9), (-9, 2), (2, 40)])
+def test_steps_and_gates_to_a_few_float32_steps(cuda_kernels, lo, hi):
+    """In halves of a float32 step: the exponential unit 4, what its argument's rounding left out 1; s = e / (2 + e) 1 + 2 + 1 more; the polynomial
+    1, its coefficients 1, what s does to it 1; the last multiply-add 1: 13 at most for a step.  A gate: 5 for the exponential, 1 + 2 for the quotient,
+    2 for products, and 1 for the output's: 11."""
+    v = (lo + (hi - lo) * torch.rand(40, 1000, generator=torch.Generator().manual_seed(hi))).to(DEV)
+    step = _few(cuda_kernels, v)
+    want = torch.logaddexp(v.double(), torch.zeros((), dtype=torch.float64, device=DEV))
+    assert float((step.double() / want - 1).abs().max()) <= 13 * 2.0 ** -24
+    ones = torch.zeros_like(v)
+    gated, plain = _few(cuda_kernels, ones, z=v), _few(cuda_kernels, ones)
+    want = plain.double() * v.double() * torch.sigmoid(v.double())
+    assert float((gated.double() - want).abs().div(want.abs()).max()) <= 11 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_steps_and_gates_far_out(cuda_kernels, dtype):
+    """No step below e^-88, the argument itself above; gates of 0 and of z; what is no number stays none."""
+    v = torch.tensor([-math.inf, -1000.0, -104.5, 50.0, 1e30, math.nan], device=DEV)[None].repeat(4, 1)
+    step = _few(cuda_kernels, v)
+    assert bool((step[:, :3] == 0).all()) and torch.equal(step[:, 3:5], v[:, 3:5]) and bool(step[:, 5].isnan().all())
+    z = torch.tensor([-3e38, -1000.0, -104.5, 0.0, 50.0, 1e30, math.nan], device=DEV)[None].repeat(4, 1).to(dtype)
+    ones = torch.zeros(4, 7, device=DEV)
+    plain, gated = _few(cuda_kernels, ones, dtype=dtype), _few(cuda_kernels, ones, z=z, dtype=dtype)
+    assert bool((gated[:, :4] == 0).all()) and torch.equal(gated[:, 4:6], (plain * z.float())[:, 4:6]) and bool(gated[:, 6].isnan().all())
