@@ -155,7 +155,8 @@ class _LayerIO(ctypes.Structure):
 
 
 class CudaKernels:
-    """Kernel table on one CUDA device."""
+    """Kernel table on one CUDA device.  Weights, and a step's arrays (spans, slots, positions, tables), may be read while the table's kernel in
+    front is still at work: results of the functions here are handed on as rows and states, not as one of those."""
 
     name = "cuda-sm100a"
     fuses_single_token_conv = True     # postnorm_add takes a short convolution for steps of single tokens
@@ -2250,7 +2251,8 @@ class CudaKernels:
         out = torch.empty(T, C, dtype=out_dtype, device=device)
         if T and R:
             longest, room, scratch = ctx.max_span, 0, None
-            # spans by stretches, as the other scans: in a bfloat16 run alone, whose sums may depend on how a span was cut into steps
+            # spans by stretches, as the other scans: in a bfloat16 run alone, whose sums may depend on how a span was cut into steps and on what else
+            # a step has
             if longest >= self.CHUNK_SCAN_MIN_SPAN and self.chunk_scans and out_dtype is torch.bfloat16:
                 room = self.lib.ifx_selective_scan_scratch(R, longest, C, N)
                 scratch = torch.empty(room, dtype=f32, device=device) if room else None

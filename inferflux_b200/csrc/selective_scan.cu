@@ -308,10 +308,10 @@ __device__ __forceinline__ int request_by_length(const int* __restrict__ cu_seql
 // up the lanes' sums over n, finish and store.
 //
 // Bound: the walk.  A token costs a channel as many exponentials as it has states (16 of them a clock and SM: 52 us for 2,048 tokens of 7,168 channels of
-// 16 states, 65 with those of steps and gates); bytes would take 23.  Measured 124 us: a walking warp issues 24 instructions a token, four of which
-// hold its exponential unit for eight clocks each, and two such warps share a scheduler with two that fetch.  Of what was measured on the way (same
-// sizes, us): walk and rows by the same warps 281, walkers apart 260 with two states a lane and 131 with four (shared memory gives a warp 128 bytes a
-// clock, and what a token's B and C cost it is the same for two states as for four); two channels a thread 150, decays four tokens ahead instead of
+// 16 states, 65 with those of steps and gates); bytes would take 23.  Measured 123 us: a walking warp issues 24 instructions a token, four of which
+// hold its exponential unit for eight clocks each, and a scheduler has two such warps, or one, beside two that fetch.  Of what was measured on the way
+// (same sizes, us): walk and rows by the same warps 281; two states a lane 165 (shared memory gives a warp 128 bytes a clock, and what a token's B
+// and C cost it is the same for two states as for four); when walkers apart took 131: two channels a thread 150, decays four tokens ahead instead of
 // two 131, a quarter of the exponentials by a polynomial 146, twice the workers 131, half of them 142.
 //
 // By stretches (what `stretch` and `pass` say): where channels are few, a span's tokens are cut into stretches of `stretch`, a block each.
@@ -632,8 +632,8 @@ __global__ void __launch_bounds__(kSpanThreads, 1) selective_span_kernel(const S
 // One token a request at most: a thread has four states of a channel of Q requests, whose rates it makes once; all its reads are under way
 // before the first is looked at (dtypes that a branch chooses are turned into float32 behind the last of them).  What there is once a
 // channel (the step, the gate, the skip, the result's way out) is done by one lane for each request, not by all of them (us: 15.0 for
-// 15.7; 24 requests 5.3 for 5.9).  WIDE: states, rates, B and C four at a time.  Bound by the states' way in and out: 64 requests of
-// 7,168 channels of 16 states, 62 MB, 15.0 us, 4.2 TB/s.
+// 15.7; 24 requests 5.3 for 5.9, before steps and gates carried what their exponential's argument was rounded by).  WIDE: states, rates, B and C four at a time.  Bound by the states' way in and out: 64 requests of
+// 7,168 channels of 16 states, 64 MB, 15.2 us, 4.2 TB/s.
 template <int LANES, bool PAD, bool WIDE, int Q>
 __global__ void __launch_bounds__(kStepThreads) selective_step_kernel(const SelectiveArgs a, int requests) {
   constexpr int S = kLaneStates, CH = kStepThreads / LANES;
@@ -828,8 +828,9 @@ static int launch_selective(SelectiveArgs a, int requests, int max_span, int str
     constexpr int kChannels = kStepThreads / LANES;
     const long long blocks = (a.channels + kChannels - 1) / kChannels;
     const bool wide = !PAD && (a.wide & 104) == 104;
-    // two requests a thread share its rates; with few requests one, for the shorter way (us, 7,168 channels: 1 request 1.6 / 1.8, 8 3.2 / 3.3, 24
-    // 7.1 / 5.3, 64 18 / 15)
+    // two requests a thread share its rates; with few requests one, for the shorter way (us, one and two a thread, 16 states, read from beyond L2: 1,024
+    // channels 12 requests 2.6 / 2.3, 24 2.9 / 3.2, 64 4.9 / 3.8; 2,048 8 2.8 / 2.9, 12 2.9 / 3.1, 64 7.6 / 5.9; 4,096 8 3.2 / 3.2, 16 4.7 / 3.7;
+    // 7,168 4 3.1 / 3.0, 8 4.3 / 3.6, 12 5.4 / 4.5, 64 20.5 / 15.8)
     constexpr int kMost = LANES >= 2 ? 2 : 1;
     const int each = requests >= 12 ? kMost : 1;
     auto kernel = each == kMost ? (wide ? selective_step_kernel<LANES, PAD, !PAD, kMost> : selective_step_kernel<LANES, PAD, false, kMost>)
@@ -880,7 +881,8 @@ extern "C" long long ifx_selective_scan_scratch(int num_requests, int max_span, 
 
 // Row strides in elements.  x and z share a dtype; bc: float32 rows of B | C; state: float32, slots slot_stride floats apart.
 // num_tokens: rows of x; cu_seqlens does not go beyond them.  A request without tokens keeps its state.  scratch: with scratch_floats of
-// ifx_selective_scan_scratch long spans may go by stretches, whose sums depend on where a span begins; null and 0: they do not.
+// ifx_selective_scan_scratch long spans may go by stretches, whose sums depend on where a span begins and on the step's other spans (their number says
+// whether there are stretches, the longest how long these are); null and 0: they do not.
 extern "C" int ifx_selective_scan(const void* x, long long ld_x, int x_dtype, const void* dt, long long ld_dt, int dt_dtype, const float* bc,
                                   long long ld_bc, const void* z, long long ld_z, const float* log_rate, const float* bias, const float* skip,
                                   float* state, long long slot_stride, const int* req_slot, const int* cu_seqlens, void* out, int out_dtype,
